@@ -52,7 +52,11 @@ typedef enum { M3G_L2 = 0, M3G_IP = 1, M3G_COSINE = 2 } m3g_metric;
 /* Element types of vectors crossing the ABI (m3g_load_cluster) and of an
  * index's list storage (m3g_create_ivf_ex).  The reference stores fp32 only
  * (Cluster::mat_, AgentMemory/M3/include/cluster.h:83). */
-typedef enum { M3G_F32 = 0, M3G_BF16 = 1 } m3g_dtype;
+typedef enum {
+    M3G_F32 = 0,
+    M3G_BF16 = 1,
+    M3G_E4M3 = 2 /* 8-bit rows of m3g_rows only: not a list storage */
+} m3g_dtype;
 #define M3G_STORE_FP32 M3G_F32
 #define M3G_STORE_BF16 M3G_BF16
 
@@ -334,6 +338,90 @@ int m3g_search_probes_device(m3g_engine* e, int index_id, const float* d_queries
 int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d_centroids,
                               int64_t nlist, int dim, int metric, int normalized, int nprobe,
                               int32_t* d_out_probes, void* stream);
+
+/* ---- Row scores: 8-bit rows, the scores themselves, scores as probabilities ----
+ *
+ * No counterpart in the reference, whose searches return the best k scores only
+ * and whose rows are fp32.  All arrays are device memory of the engine's device.
+ * The calls use no index and no scratch of the engine, so calls on several
+ * streams may overlap, and each may be captured into a CUDA graph (make one call
+ * of these before the first capture: it allocates the engine's error word).
+ * Enqueued on `stream`; stream NULL: the legacy default stream, waited for.  What
+ * a kernel finds wrong on the device (a pair or list out of range, a wait that
+ * gave up) is left out and reported by m3g_sync_errors, or by the call itself
+ * when it waits.  Inputs and outputs must not overlap.
+ *
+ * Rows of vectors, one row every `ld` elements:
+ *   M3G_BF16  data holds uint16 bf16 bit patterns; scales is not used;
+ *   M3G_E4M3  data holds 8-bit e4m3 codes (1 sign, 4 exponent, 3 mantissa bits,
+ *             no infinity); scales [n, ld_scales] holds one byte s per 128 dims:
+ *             dim i stands for code * 2^(s[i / 128] - 127); s = 255 is not a scale.
+ * data starts on a 16-byte boundary and ld is a multiple of 16 bytes; scales
+ * starts on a 4-byte boundary and ld_scales is a multiple of 4, at least
+ * ceil(dim / 128).  n < 2^31. */
+typedef struct {
+    const void* data;
+    const uint8_t* scales;
+    int64_t n, ld, ld_scales;
+    int32_t dim, dtype;
+} m3g_rows;
+
+/* Packs rows x [n, dim] (one every ldx elements; M3G_F32 or M3G_BF16) into the
+ * codes and scales of `out` (dtype M3G_E4M3, n and dim as given; both arrays are
+ * written).  The scale of 128 dims is the least 2^e, e >= -126, with
+ * |x| <= 448 * 2^e for their finite values; the code is x / 2^e rounded to
+ * nearest even (a relative error of at most 2^-4 where |x| >= 2^-6 * 2^e).
+ * An infinity is kept as +-448 * 2^e, a NaN as NaN.  Bytes past dim and past
+ * ceil(dim / 128) in a row are not written. */
+int m3g_pack_rows_device(m3g_engine* e, const void* d_x, int dtype, int64_t n, int dim,
+                         int64_t ldx, const m3g_rows* out, void* stream);
+
+/* out[i * ld_out + j] = alpha * <q_i, x_j> + beta for every row i of q and j of x
+ * (same dtype and dim), in out_dtype M3G_F32 or M3G_BF16.  Products and sums are
+ * fp32; beta = 0 or alpha = -1 give the inner product and the engine's IP score,
+ * alpha = -1, beta = 1 its COSINE score of normalized rows.  ld_out >= x->n. */
+int m3g_row_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, float alpha,
+                          float beta, void* d_out, int out_dtype, int64_t ld_out, void* stream);
+
+/* The scores of every row of each query's probed lists (products grouped by
+ * list, ragged on both sides).  List g holds rows d_list_off[g] ..
+ * d_list_off[g] + d_list_len[g] - 1 of x; pairs d_pair_off[g] ..
+ * d_pair_off[g + 1] - 1 are the queries that probe it; pair p is row
+ * d_pair_row[p] of q (row p where d_pair_row is null; -1 skips the pair) and
+ * writes d_list_len[g] scores alpha * <q, x> + beta to d_out from element
+ * d_out_off[p] on (elements no pair writes keep their values; pairs must not
+ * share elements).  d_pair_off [ngroup + 1] ascending from 0 to npair.  out_n:
+ * the elements of d_out; pairs whose scores would end past it are left out and
+ * reported, as are lists and pairs out of range. */
+int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, int64_t ngroup,
+                           const int64_t* d_list_off, const int32_t* d_list_len,
+                           const int64_t* d_pair_off, int64_t npair, const int32_t* d_pair_row,
+                           const int64_t* d_out_off, float alpha, float beta, void* d_out,
+                           int out_dtype, int64_t out_n, void* stream);
+
+/* Scores as probabilities: row i of the scores (dtype M3G_F32 or M3G_BF16) is n
+ * entries from element i * ld on, or, with d_row_off [nq + 1] ascending, entries
+ * d_row_off[i] .. d_row_off[i + 1] - 1 of n entries in all (ld is not used).  With
+ * l = scale * score (scale finite and not 0), over the entries whose l is neither
+ * NaN nor -inf (the others are left out: they have no probability):
+ *   out_logsumexp[i] = log sum exp(l)               (-inf where no entry is left)
+ *   out_entropy[i]   = -sum p log p, p = exp(l - logsumexp)   (0 there)
+ *   out_given[i, j]  = log p of entry d_given[i, j] (its place in the row) of ngiven
+ *                      given ones; -inf for one left out or outside the row
+ *   out_top[i, 0..k-1], out_top_index[i, ..] = the k largest log p, largest first,
+ *                      and their places in the row (scores that are equal: the
+ *                      lower place first); -inf and -1 past the last entry.
+ * k <= 128 (M3G_EUNSUPPORTED above).  ngiven or k may be 0 (their arrays null).
+ * A l of +inf gives logsumexp +inf and entropy NaN.  d_work holds work_bytes >=
+ * m3g_score_probs_work() bytes on an 8-byte boundary (null where that is 0): scratch
+ * of this call, which calls that overlap must not share. */
+int m3g_score_probs_work(m3g_engine* e, int64_t nq, int64_t n, int ragged, int k,
+                         int64_t* out_bytes);
+int m3g_score_probs_device(m3g_engine* e, const void* d_scores, int dtype, int64_t nq, int64_t n,
+                           int64_t ld, const int64_t* d_row_off, float scale,
+                           const int64_t* d_given, int ngiven, int k, float* d_out_logsumexp,
+                           float* d_out_entropy, float* d_out_given, int64_t* d_out_top_index,
+                           float* d_out_top, void* d_work, int64_t work_bytes, void* stream);
 
 /* Test hook for the device-side failure path: with ns > 0, every tensor-core
  * list scan first waits up to ns nanoseconds on a barrier that nothing

@@ -17,6 +17,7 @@ M3G_OK, M3G_EINVAL, M3G_ERANGE, M3G_ERUNTIME, M3G_ECUDA, M3G_ENCCL, M3G_ETIMEOUT
     M3G_EUNSUPPORTED = range(8)
 L2, IP, COSINE = 0, 1, 2
 F32, BF16 = 0, 1  # m3g_dtype: vector element types and list storage
+E4M3 = 2  # m3g_dtype of 8-bit rows (m3g_rows)
 
 
 def bf16_bits(x):
@@ -48,6 +49,13 @@ class Profile(ct.Structure):
                 ("kernel_launches", ct.c_int32), ("nq", ct.c_int32), ("nprobe", ct.c_int32),
                 ("k", ct.c_int32), ("graph_launches", ct.c_int64),
                 ("graph_capture_failures", ct.c_int64), ("streamed_bytes", ct.c_int64)]
+
+
+class Rows(ct.Structure):
+    """m3g_rows: rows of bf16 values, or of e4m3 codes with their scale bytes."""
+    _fields_ = [("data", ct.c_void_p), ("scales", ct.c_void_p), ("n", ct.c_int64),
+                ("ld", ct.c_int64), ("ld_scales", ct.c_int64), ("dim", ct.c_int32),
+                ("dtype", ct.c_int32)]
 
 
 SIGNATURES = {
@@ -108,6 +116,15 @@ SIGNATURES = {
     "m3g_load_index": (_i32, [_vp, _i32, ct.c_char_p]),
     "m3g_select_probes_noalloc": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp,
                                          _vp]),
+    "m3g_pack_rows_device": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, ct.POINTER(Rows), _vp]),
+    "m3g_row_scores_device": (_i32, [_vp, ct.POINTER(Rows), ct.POINTER(Rows), ct.c_float,
+                                     ct.c_float, _vp, _i32, _i64, _vp]),
+    "m3g_list_scores_device": (_i32, [_vp, ct.POINTER(Rows), ct.POINTER(Rows), _i64, _vp, _vp,
+                                      _vp, _i64, _vp, _vp, ct.c_float, ct.c_float, _vp, _i32,
+                                      _i64, _vp]),
+    "m3g_score_probs_work": (_i32, [_vp, _i64, _i64, _i32, _i32, _pi64]),
+    "m3g_score_probs_device": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _vp, ct.c_float, _vp,
+                                      _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "m3g_set_profiling": (_i32, [_vp, _i32]),
     "m3g_last_profile": (_i32, [_vp, ct.POINTER(Profile)]),
 }
@@ -459,6 +476,35 @@ class Engine:
                                              ct.c_void_p(probes_ptr), nprobe, ct.c_void_p(ids_ptr),
                                              ct.c_void_p(scores_ptr), ct.c_void_p(counts_ptr),
                                              ct.c_void_p(stream) if stream else None))
+
+    # row scores (device pointers; Rows describes packed or bf16 rows).  The torch
+    # form of these calls is m3_memory_b200.row_scores.
+    def pack_rows_device(self, x_ptr, dtype, n, dim, ldx, out, stream=None):
+        check(lib().m3g_pack_rows_device(self.h, x_ptr, dtype, n, dim, ldx, out, stream))
+
+    def row_scores_device(self, q, x, alpha, beta, out_ptr, out_dtype, ld_out, stream=None):
+        check(lib().m3g_row_scores_device(self.h, q, x, alpha, beta, out_ptr, out_dtype, ld_out,
+                                          stream))
+
+    def list_scores_device(self, q, x, ngroup, list_off_ptr, list_len_ptr, pair_off_ptr, npair,
+                           pair_row_ptr, out_off_ptr, alpha, beta, out_ptr, out_dtype, out_n,
+                           stream=None):
+        check(lib().m3g_list_scores_device(self.h, q, x, ngroup, list_off_ptr, list_len_ptr,
+                                           pair_off_ptr, npair, pair_row_ptr, out_off_ptr, alpha,
+                                           beta, out_ptr, out_dtype, out_n, stream))
+
+    def score_probs_work(self, nq, n, ragged, k):
+        out = ct.c_int64()
+        check(lib().m3g_score_probs_work(self.h, nq, n, int(ragged), k, ct.byref(out)))
+        return out.value
+
+    def score_probs_device(self, scores_ptr, dtype, nq, n, ld, row_off_ptr, scale, given_ptr,
+                           ngiven, k, lse_ptr, entropy_ptr, out_given_ptr, top_index_ptr, top_ptr,
+                           work_ptr, work_bytes, stream=None):
+        check(lib().m3g_score_probs_device(self.h, scores_ptr, dtype, nq, n, ld, row_off_ptr,
+                                           scale, given_ptr, ngiven, k, lse_ptr, entropy_ptr,
+                                           out_given_ptr, top_index_ptr, top_ptr, work_ptr,
+                                           work_bytes, stream))
 
     def sync_errors(self):
         check(lib().m3g_sync_errors(self.h))

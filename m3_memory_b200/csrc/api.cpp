@@ -496,6 +496,81 @@ int m3g_search_probes_device(m3g_engine* e, int index_id, const float* d_queries
     });
 }
 
+int m3g_pack_rows_device(m3g_engine* e, const void* d_x, int dtype, int64_t n, int dim,
+                         int64_t ldx, const m3g_rows* out, void* stream) {
+    M3G_ENGINE_OR_FAIL(e);
+    return guarded([&] {
+        e->eng.pack_rows(d_x, dtype, n, dim, ldx, out, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int m3g_row_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, float alpha,
+                          float beta, void* d_out, int out_dtype, int64_t ld_out, void* stream) {
+    M3G_ENGINE_OR_FAIL(e);
+    return guarded([&] {
+        e->eng.row_scores(q, x, alpha, beta, d_out, out_dtype, ld_out,
+                          static_cast<cudaStream_t>(stream));
+    });
+}
+
+int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, int64_t ngroup,
+                           const int64_t* d_list_off, const int32_t* d_list_len,
+                           const int64_t* d_pair_off, int64_t npair, const int32_t* d_pair_row,
+                           const int64_t* d_out_off, float alpha, float beta, void* d_out,
+                           int out_dtype, int64_t out_n, void* stream) {
+    M3G_ENGINE_OR_FAIL(e);
+    return guarded([&] {
+        m3g::ScoreGroups g;
+        g.ngroup = ngroup;
+        g.npair = npair;
+        g.out_n = out_n;
+        g.list_off = d_list_off;
+        g.list_len = d_list_len;
+        g.pair_off = d_pair_off;
+        g.pair_row = d_pair_row;
+        g.out_off = d_out_off;
+        e->eng.list_scores(q, x, g, alpha, beta, d_out, out_dtype,
+                           static_cast<cudaStream_t>(stream));
+    });
+}
+
+int m3g_score_probs_work(m3g_engine* e, int64_t nq, int64_t n, int ragged, int k,
+                         int64_t* out_bytes) {
+    M3G_ENGINE_OR_FAIL(e);
+    return guarded([&] {
+        if (!out_bytes) m3g::fail(M3G_EINVAL, "score_probs_work: out missing");
+        *out_bytes = e->eng.score_probs_work(nq, n, ragged != 0, k);
+    });
+}
+
+int m3g_score_probs_device(m3g_engine* e, const void* d_scores, int dtype, int64_t nq, int64_t n,
+                           int64_t ld, const int64_t* d_row_off, float scale,
+                           const int64_t* d_given, int ngiven, int k, float* d_out_logsumexp,
+                           float* d_out_entropy, float* d_out_given, int64_t* d_out_top_index,
+                           float* d_out_top, void* d_work, int64_t work_bytes, void* stream) {
+    M3G_ENGINE_OR_FAIL(e);
+    return guarded([&] {
+        m3g::ProbsArgs a{};
+        a.scores = d_scores;
+        a.dtype = dtype;
+        a.nq = nq;
+        a.n = n;
+        a.ld = ld;
+        a.row_off = d_row_off;
+        a.scale = scale;
+        a.given = d_given;
+        a.ngiven = ngiven;
+        a.k = k;
+        a.lse = d_out_logsumexp;
+        a.entropy = d_out_entropy;
+        a.out_given = d_out_given;
+        a.top_index = d_out_top_index;
+        a.top = d_out_top;
+        a.work = d_work;
+        e->eng.score_probs(a, work_bytes, static_cast<cudaStream_t>(stream));
+    });
+}
+
 int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d_centroids,
                               int64_t nlist, int dim, int metric, int normalized, int nprobe,
                               int32_t* d_out_probes, void* stream) {

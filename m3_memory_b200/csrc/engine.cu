@@ -811,7 +811,9 @@ void Engine::set_device(int dev) {
     M3G_CK(cudaGetDeviceCount(&count));
     if (dev < 0 || dev >= count) fail(M3G_EINVAL, "set_device: no such CUDA device");
     std::shared_lock lk(imu_);
-    if (!indices_.empty() || ws_.stream) fail(M3G_ERUNTIME, "set_device: engine already in use");
+    std::lock_guard sl(score_mu_);
+    if (!indices_.empty() || ws_.stream || score_err_.p)
+        fail(M3G_ERUNTIME, "set_device: engine already in use");
     device_ = dev;
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device_) == cudaSuccess && n > 0)
@@ -1977,6 +1979,7 @@ void Engine::search(int index_id, const float* Q, int64_t nq, int k, int nprobe,
 
 void Engine::sync_errors() {
     DeviceGuard g(device_);
+    row_score_errors();
     std::lock_guard wl(ws_.mu);
     if (!ws_.stream) return;
     M3G_CK(cudaEventSynchronize(ws_.done));

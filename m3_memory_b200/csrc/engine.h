@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "kernels_scores.h"
 #include "m3gpu.h"
 
 namespace m3g {
@@ -251,6 +252,17 @@ class Engine {
                           bool on_device = false);
     void sync_errors();
 
+    // Row scores (row_scores.cpp): device pointers, enqueued on ext_stream (null: the
+    // legacy default stream, waited for).  They use no index and no workspace.
+    void pack_rows(const void* dX, int dtype, int64_t n, int dim, int64_t ldx, const m3g_rows* out,
+                   cudaStream_t ext_stream);
+    void row_scores(const m3g_rows* q, const m3g_rows* x, float alpha, float beta, void* d_out,
+                    int out_dtype, int64_t ld_out, cudaStream_t ext_stream);
+    void list_scores(const m3g_rows* q, const m3g_rows* x, const ScoreGroups& groups, float alpha,
+                     float beta, void* d_out, int out_dtype, cudaStream_t ext_stream);
+    int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int k);
+    void score_probs(const ProbsArgs& a, int64_t work_bytes, cudaStream_t ext_stream);
+
     void info(int index_id, int* dim, int* metric, int* normalized, int* nlist);
     void cluster_size(int index_id, int cid, int64_t* size, int64_t* live);
     void get_centroids(int index_id, float* out);
@@ -337,6 +349,13 @@ class Engine {
     std::mutex err_mu_;
     std::string first_error_;
     int first_error_code_ = 0;
+
+    // error words of the row-score calls (kScoreErrWords ints on the device, made by
+    // the first call); row_score_errors() reads and clears them
+    int* score_err();
+    void row_score_errors();
+    std::mutex score_mu_;
+    DBuf<int> score_err_;
 
     Workspace ws_;
     std::atomic<bool> profiling_{false};

@@ -1,0 +1,53 @@
+// kernels_scores.h -- launchers of the row-score kernels (k_scores.cu, k_probs.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "m3gpu.h"
+
+namespace m3g {
+
+constexpr int kScaleDims = 128;  // dims that share one scale byte
+
+// Error words of the row-score calls (one pair per engine).
+enum ScoreError : int { kScoreTimeout = 0, kScoreBadItem = 1, kScoreErrWords = 2 };
+
+// The group form's lists and pairs (all null / 0 in the dense form).
+struct ScoreGroups {
+    int64_t ngroup = 0, npair = 0, out_n = 0;
+    const int64_t* list_off = nullptr;
+    const int32_t* list_len = nullptr;
+    const int64_t* pair_off = nullptr;
+    const int32_t* pair_row = nullptr;
+    const int64_t* out_off = nullptr;
+};
+
+cudaError_t launch_pack_rows(const void* x, int dtype, int64_t n, int dim, int64_t ldx,
+                             uint8_t* codes, int64_t ld, uint8_t* scales, int64_t lds,
+                             cudaStream_t st);
+cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
+                              void* out, int out_dtype, int64_t ld_out, int* err, int sms,
+                              cudaStream_t st);
+cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const ScoreGroups& g,
+                               float alpha, float beta, void* out, int out_dtype, int* err,
+                               int sms, cudaStream_t st);
+
+constexpr int kProbsMaxK = 128;
+int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int k, int sms);
+struct ProbsArgs {
+    const void* scores;
+    int dtype;
+    int64_t nq, n, ld;
+    const int64_t* row_off;
+    float scale;
+    const int64_t* given;
+    int ngiven, k;
+    float *lse, *entropy, *out_given;
+    int64_t* top_index;
+    float* top;
+    void* work;
+};
+cudaError_t launch_score_probs(const ProbsArgs& a, int sms, cudaStream_t st);
+
+}  // namespace m3g
