@@ -1,0 +1,640 @@
+// k_scores_tc.cu -- scores of queries against rows on the tensor cores: every row
+// (dense) or the rows of each query's probed lists (grouped, ragged both ways).
+//
+// out[pair][j] = alpha * sum_i q_i x_ji + beta.  The rows lie along the MMA's M
+// (128 rows of x a tile) and the queries along N, so a tile takes just as many
+// columns as its list has queries (16 .. NT, a multiple of 16): with few queries a
+// list the rows' bytes bound the kernel, and padding the queries to 128 would
+// triple the operand traffic.  TMEM then holds one row of x per lane and one query
+// per column, so a warp stores 32 neighbouring scores of one query: full lines
+// without a detour through shared memory.
+//
+// 8-bit rows use kind::mxf8f6f4 with block scales: the hardware multiplies each
+// 32-deep product by 2^(sx + sq - 254), both scale bytes read from TMEM.  One byte
+// covers 128 dims, so the four MMAs of a 128-byte slice share it, and the four
+// slices of a 512-dim chunk take bytes 0..3 of the same TMEM words.  bf16 rows use
+// kind::f16.  Sums are fp32 in TMEM.
+//
+// A launch is one CTA per SM, each with an equal run of consecutive tiles (group,
+// 128 rows, up to NT queries; queries fastest, so the rows come from L2 after their
+// first tile).  Warp 0 loads (TMA; queries of a group by gather4), warp 1 issues
+// the MMAs, warp 2 brings scale words, warp 3 walks the groups and queues tiles,
+// warps 4-7 store.  Every wait is bounded.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "kernels_scores.h"
+#include "tc.cuh"
+
+namespace m3g {
+namespace {
+
+constexpr int kM = 128;                 // rows of x a tile
+constexpr int kSlice = 128;             // bytes of a row a stage (128 8-bit or 64 bf16 dims)
+constexpr int kXBytes = kM * kSlice;
+constexpr int kThreads = 256;
+constexpr int kEpi0 = 4;                // first epilogue warp
+constexpr int kItems = 4;               // tiles queued ahead
+constexpr int kEpiBar = 1;              // named barriers of the epilogue warps: this and the next
+
+// The two launch shapes: up to 64 queries a tile with eight stages in flight, for
+// rows that are read for a few queries each, and up to 240 with four.
+template <int NT>
+struct Shape;
+template <>
+struct Shape<64> {
+    static constexpr int kStages = 8, kBox = 16, kAcc = 64, kTmem = 256, kSf0 = 128, kSfStep = 16;
+};
+template <>
+struct Shape<240> {  // each accumulator's scales in the 16 columns behind it
+    static constexpr int kStages = 4, kBox = 48, kAcc = 256, kTmem = 512, kSf0 = 240,
+                         kSfStep = 256;
+};
+
+struct Item {
+    int32_t x0, nx;  // first row of x, rows (0: no more tiles)
+    int32_t q0, nq;  // first pair, pairs
+    int64_t j0;      // the first row's place in its list
+};
+
+constexpr int kSfBytes = 512 + 1024;  // scale words of a 512-dim chunk: x rows, queries
+
+template <int NT>
+struct alignas(1024) Smem {
+    unsigned char stage[Shape<NT>::kStages][kXBytes + NT * kSlice];
+    unsigned char sf[2][kSfBytes];
+    int64_t base[2][NT];  // where each column's scores start; -1: nowhere
+    int64_t prefix[kThreads + 1];
+    Item items[kItems];
+    uint64_t full[Shape<NT>::kStages], empty[Shape<NT>::kStages];
+    uint64_t accfull[2], accempty[2], sffull[2], sfempty[2];
+    uint64_t itemfull[kItems], itemempty[kItems], drain;
+    int64_t warp_sum[kThreads / 32];
+    uint32_t tmem;
+    int abort;
+};
+
+struct Params {
+    int64_t nq, nx;  // rows of q and x
+    int nk;          // slices of a row
+    int row_bytes;   // bytes of a row that hold dims
+    const uint8_t *qs, *xs;
+    int64_t lqs, lxs;
+    float alpha, beta;
+    int64_t ld_out;  // dense form
+    ScoreGroups g;   // group form
+    int* err;
+};
+
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, int r0,
+                                            int r1, int r2, int r3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t sfa, uint32_t sfb, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X "
+        "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+// 32 rows of 16 bytes from shared memory to four TMEM columns, repeated in each of
+// the four lane quarters: the words of rows r, r + 32, r + 64, r + 96 are row r's 16
+// bytes.  No swizzle; 8 rows of 16 bytes every 128 bytes.
+__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint32_t saddr) {
+    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(128 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d)
+                 : "memory");
+}
+
+// kind::mxf8f6f4: both operands e4m3 (0) and K-major, N >> 3 at bits 17-22, ue8m0
+// scales (bit 23), M >> 7 at bits 27-28; the scale byte of the words: bits 4-5 (B)
+// and 29-30 (A).
+__device__ __forceinline__ uint32_t mx_idesc(int n, int byte) {
+    return ((uint32_t)byte << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27) |
+           ((uint32_t)byte << 29);
+}
+
+// A group's tiles: its rows in 128s times its pairs in nqt parts of `per`.
+template <int NT>
+__device__ __forceinline__ int64_t group_tiles(int64_t len, int64_t m, int* per, int* nqt) {
+    *per = NT;
+    *nqt = 0;
+    if (len <= 0 || m <= 0) return 0;
+    const int64_t parts = (m + NT - 1) / NT;
+    *per = (int)((((m + parts - 1) / parts) + 15) / 16 * 16);
+    *nqt = (int)((m + *per - 1) / *per);
+    return (len + kM - 1) / kM * *nqt;
+}
+
+// The group's rows and pairs; false (and nothing in it) when they are out of range.
+struct GroupAt {
+    int64_t l0, len, p0, m;
+};
+__device__ __forceinline__ bool load_group(const Params& p, int64_t i, GroupAt* o) {
+    const ScoreGroups& g = p.g;
+    const int64_t a = g.pair_off[i], b = g.pair_off[i + 1];
+    o->l0 = g.list_off[i];
+    o->len = g.list_len[i];
+    o->p0 = a;
+    o->m = b - a;
+    const bool bad = a < 0 || b < a || b > g.npair || o->len < 0 || o->l0 < 0 ||
+                     o->l0 > p.nx || o->len > p.nx - o->l0;
+    if (bad) o->len = o->m = 0;
+    return !bad || a == b;
+}
+
+template <bool F8, int NT, bool GROUP, class O>
+__global__ void __launch_bounds__(kThreads, 1)
+    scores_tc_kernel(const __grid_constant__ CUtensorMap map_x,
+                     const __grid_constant__ CUtensorMap map_x32,
+                     const __grid_constant__ CUtensorMap map_q, O* __restrict__ out,
+                     const __grid_constant__ Params p) {
+    using S = Shape<NT>;
+    extern __shared__ unsigned char smem_raw[];
+    Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (warp == 0) tmem_alloc(&sm.tmem, S::kTmem);
+    if (threadIdx.x == 32) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&sm.accfull[s], 1);
+            mbar_init(&sm.accempty[s], 4);
+            mbar_init(&sm.sffull[s], 1);
+            mbar_init(&sm.sfempty[s], 1);
+        }
+        for (int s = 0; s < kItems; ++s) {
+            mbar_init(&sm.itemfull[s], 1);
+            mbar_init(&sm.itemempty[s], F8 ? 7 : 6);  // warps 0, 1, (2,) 4-7
+        }
+        mbar_init(&sm.drain, 1);
+        sm.abort = 0;
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&map_x);
+        prefetch_tensormap(&map_x32);
+        prefetch_tensormap(&map_q);
+    }
+
+    // This CTA's run of tiles.  Grouped: the tiles of all groups are counted first,
+    // each thread a run of groups.
+    int64_t total;
+    int64_t chunk = 0;  // groups a thread counts
+    if constexpr (GROUP) {
+        chunk = (p.g.ngroup + kThreads - 1) / kThreads;
+        const int64_t g0 = chunk * threadIdx.x, g1 = min(g0 + chunk, p.g.ngroup);
+        int64_t mine = 0;
+        bool ok = true;
+        for (int64_t i = g0; i < g1; ++i) {
+            GroupAt at;
+            int per, nqt;
+            ok &= load_group(p, i, &at);
+            mine += group_tiles<NT>(at.len, at.m, &per, &nqt);
+        }
+        if (!ok && blockIdx.x == 0) atomicOr(p.err + kScoreBadItem, 1);
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) sm.warp_sum[warp] = incl;
+        __syncthreads();
+        int64_t before = 0;
+        for (int w = 0; w < warp; ++w) before += sm.warp_sum[w];
+        sm.prefix[threadIdx.x] = before + incl - mine;
+        if (threadIdx.x == kThreads - 1) sm.prefix[kThreads] = before + incl;
+    } else {
+        int per, nqt;
+        total = group_tiles<NT>(p.nx, p.nq, &per, &nqt);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if constexpr (GROUP) total = sm.prefix[kThreads];
+    const int64_t share = total / gridDim.x, more = total % gridDim.x;
+    const int64_t t0 = share * blockIdx.x + min((int64_t)blockIdx.x, more);
+    const int64_t t1 = t0 + share + ((int64_t)blockIdx.x < more ? 1 : 0);
+    const uint32_t tmem = sm.tmem;
+
+    // The next queued tile; false: none left, or the launch gave up.
+    auto next_item = [&](int64_t i, Item* it) {
+        const int s = (int)(i % kItems);
+        const bool ok = mbar_wait(&sm.itemfull[s], (uint32_t)(i / kItems) & 1u, &sm.abort);
+        if (ok) *it = sm.items[s];
+        __syncwarp();
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (lane == 0) mbar_arrive(&sm.itemempty[s]);
+        return it->nx > 0;
+    };
+    auto columns = [](const Item& it) { return (it.nq + 15) & ~15; };
+
+    if (warp == 0) {
+        // ---- loads
+        int64_t it = 0;
+        bool ok = true;
+        Item item;
+        for (int64_t i = 0; ok && next_item(i, &item); ++i) {
+            const int n = columns(item);
+            int rows[2][4];  // the rows of gathers lane and lane + 32
+            uint32_t qbytes;
+            const bool gather = GROUP && p.g.pair_row != nullptr;
+            if (gather) {
+#pragma unroll
+                for (int h = 0; h < (NT > 128 ? 2 : 1); ++h)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int c = 4 * (lane + 32 * h) + u;
+                        const int r = c < item.nq ? p.g.pair_row[item.q0 + c] : 0;
+                        rows[h][u] = r >= 0 && r < p.nq ? r : 0;
+                    }
+                qbytes = (uint32_t)n * kSlice;
+            } else {
+                qbytes = (uint32_t)((n + S::kBox - 1) / S::kBox * S::kBox) * kSlice;
+            }
+            const int xboxes = item.nx > 96 ? 0 : (item.nx + 31) / 32;
+            const uint32_t bytes = qbytes + (xboxes ? (uint32_t)xboxes * 32 * kSlice : kXBytes);
+            for (int kt = 0; kt < p.nk; ++kt, ++it) {
+                const int s = (int)(it % S::kStages);
+                if (it >= S::kStages)
+                    ok = mbar_wait(&sm.empty[s], (uint32_t)((it / S::kStages) - 1) & 1u,
+                                   &sm.abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                unsigned char* sx = sm.stage[s];
+                unsigned char* sq = sx + kXBytes;
+                const int x = kt * (F8 ? kSlice : kSlice / 2);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sm.full[s], bytes);
+                    if (xboxes == 0) {
+                        tma_load_2d(sx, &map_x, x, item.x0, &sm.full[s]);
+                    } else {
+                        for (int b = 0; b < xboxes; ++b)
+                            tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b,
+                                        &sm.full[s]);
+                    }
+                    if (!gather)
+                        for (int b = 0; b * S::kBox < n; ++b)
+                            tma_load_2d(sq + b * S::kBox * kSlice, &map_q, x,
+                                        item.q0 + b * S::kBox, &sm.full[s]);
+                }
+                __syncwarp();
+                if (gather) {
+#pragma unroll
+                    for (int h = 0; h < (NT > 128 ? 2 : 1); ++h) {
+                        const int c = 4 * (lane + 32 * h);
+                        if (c < n)
+                            tma_gather4(sq + c * kSlice, &map_q, x, rows[h][0], rows[h][1],
+                                        rows[h][2], rows[h][3], &sm.full[s]);
+                    }
+                }
+            }
+        }
+        // no copy may still be landing when the CTA leaves
+        if (lane == 0)
+            for (int64_t k = it > S::kStages ? it - S::kStages : 0; k < it; ++k)
+                mbar_drain(&sm.full[k % S::kStages], (uint32_t)(k / S::kStages) & 1u);
+    } else if (warp == 1) {
+        // ---- MMAs: tile i accumulates in TMEM half i & 1
+        int64_t it = 0, sf = 0;
+        bool ok = true;
+        Item item;
+        for (int64_t i = 0; ok && next_item(i, &item); ++i) {
+            const int h = (int)(i & 1), n = columns(item);
+            if (i >= 2)
+                ok = mbar_wait(&sm.accempty[h], (uint32_t)((i >> 1) - 1) & 1u, &sm.abort);
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(h * S::kAcc);
+            for (int kt = 0; ok && kt < p.nk; ++kt, ++it) {
+                const int s = (int)(it % S::kStages);
+                const int c = (int)(sf & 1);
+                const uint32_t tsf = tmem + (uint32_t)(S::kSf0 + c * S::kSfStep);
+                if (F8 && (kt & 3) == 0)
+                    ok = mbar_wait(&sm.sffull[c], (uint32_t)(sf >> 1) & 1u, &sm.abort);
+                ok = ok && mbar_wait(&sm.full[s], (uint32_t)(it / S::kStages) & 1u, &sm.abort);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    if (F8 && (kt & 3) == 0) {
+                        const uint32_t src = smem_u32(sm.sf[c]);
+                        tc_copy_scales(tsf, src);
+                        tc_copy_scales(tsf + 4, src + 512);
+                        if (NT > 128) tc_copy_scales(tsf + 8, src + 1024);
+                    }
+                    const uint32_t sx = smem_u32(sm.stage[s]), sq = sx + kXBytes;
+                    const int left = (p.row_bytes - kt * kSlice + 31) / 32;  // 32-byte steps
+#pragma unroll
+                    for (int k = 0; k < kSlice / 32; ++k) {
+                        if (k >= left) break;
+                        const uint64_t a = sw128_desc(sx + k * 32), b = sw128_desc(sq + k * 32);
+                        if (F8)
+                            tc_mma_mx(d, a, b, mx_idesc(n, kt & 3), tsf, tsf + 4, (kt | k) != 0);
+                        else
+                            tc_mma_f16(d, a, b, tc_idesc_m128(n, 1), (kt | k) != 0);
+                    }
+                    tc_commit(&sm.empty[s]);
+                    if (F8 && ((kt & 3) == 3 || kt + 1 == p.nk)) tc_commit(&sm.sfempty[c]);
+                    if (kt + 1 == p.nk) tc_commit(&sm.accfull[h]);
+                }
+                if (F8 && ((kt & 3) == 3 || kt + 1 == p.nk)) ++sf;
+                __syncwarp();
+            }
+            ok = __all_sync(0xffffffffu, ok);
+        }
+        if (lane == 0) {
+            // fires once every MMA issued above has completed (also on an error path)
+            tc_commit(&sm.drain);
+            mbar_drain(&sm.drain, 0);
+        }
+    } else if (warp == 2) {
+        if constexpr (F8) {
+            // ---- scale words: lane r brings rows r, r + 32, ..; the slot of chunk c
+            // is free in shared memory and in TMEM once chunk c - 2's MMAs are done
+            int64_t sf = 0;
+            bool ok = true;
+            Item item;
+            for (int64_t i = 0; ok && next_item(i, &item); ++i) {
+                const uint8_t *xp[4], *qp[NT > 128 ? 8 : 4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int r = lane + 32 * u;
+                    xp[u] = r < item.nx ? p.xs + (item.x0 + r) * p.lxs : nullptr;
+                }
+#pragma unroll
+                for (int u = 0; u < (NT > 128 ? 8 : 4); ++u) {
+                    const int c = lane + 32 * u;
+                    qp[u] = nullptr;
+                    if (c < item.nq) {
+                        int64_t r = (int64_t)item.q0 + c;
+                        if (GROUP && p.g.pair_row) r = p.g.pair_row[r];
+                        if (r >= 0 && r < p.nq) qp[u] = p.qs + r * p.lqs;
+                    }
+                }
+                for (int kt = 0; kt < p.nk; kt += 4, ++sf) {
+                    const uint32_t one = 0x7F7F7F7Fu;
+                    uint32_t w[4 + (NT > 128 ? 8 : 4)];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        w[u] = xp[u] ? __ldg(reinterpret_cast<const uint32_t*>(xp[u] + kt)) : one;
+#pragma unroll
+                    for (int u = 0; u < (NT > 128 ? 8 : 4); ++u)
+                        w[4 + u] =
+                            qp[u] ? __ldg(reinterpret_cast<const uint32_t*>(qp[u] + kt)) : one;
+                    const int c = (int)(sf & 1);
+                    if (sf >= 2)
+                        ok = mbar_wait(&sm.sfempty[c], (uint32_t)((sf >> 1) - 1) & 1u, &sm.abort);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+#pragma unroll
+                    for (int u = 0; u < 4 + (NT > 128 ? 8 : 4); u += 4)
+                        *reinterpret_cast<uint4*>(sm.sf[c] + 128 * u + 16 * lane) =
+                            make_uint4(w[u], w[u + 1], w[u + 2], w[u + 3]);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.sffull[c]);
+                }
+            }
+        }
+    } else if (warp == 3) {
+        // ---- tiles t0 .. t1 - 1, 32 groups at a time, queued for the others
+        int64_t i = 0;
+        bool ok = true;
+        auto queue = [&](const Item& item) {
+            const int s = (int)(i % kItems);
+            if (i >= kItems)
+                ok = mbar_wait(&sm.itemempty[s], (uint32_t)((i / kItems) - 1) & 1u, &sm.abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            if (lane == 0) {
+                sm.items[s] = item;
+                mbar_arrive(&sm.itemfull[s]);
+            }
+            __syncwarp();
+            ++i;
+        };
+        auto queue_group = [&](const GroupAt& at, int64_t first, int64_t from, int64_t to) {
+            // tiles from .. to - 1 of the launch, of the group whose first one is `first`
+            int per, nqt;
+            group_tiles<NT>(at.len, at.m, &per, &nqt);
+            for (int64_t t = from; ok && t < to; ++t) {
+                const int64_t xt = (t - first) / nqt, qt = (t - first) % nqt;
+                Item item;
+                item.j0 = xt * kM;
+                item.x0 = (int32_t)(at.l0 + item.j0);
+                item.nx = (int32_t)min((int64_t)kM, at.len - item.j0);
+                item.q0 = (int32_t)(at.p0 + qt * per);
+                item.nq = (int32_t)min((int64_t)per, at.m - qt * per);
+                queue(item);
+            }
+        };
+        if constexpr (GROUP) {
+            if (t0 < t1) {
+                int lo = 0, hi = kThreads;  // the last run that starts at or before t0
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (sm.prefix[mid] <= t0) lo = mid;
+                    else hi = mid;
+                }
+                int64_t first = sm.prefix[lo];
+                for (int64_t g = lo * chunk; ok && g < p.g.ngroup && first < t1; g += 32) {
+                    GroupAt at{0, 0, 0, 0};
+                    int per, nqt;
+                    if (g + lane < p.g.ngroup) load_group(p, g + lane, &at);
+                    const int64_t tiles = group_tiles<NT>(at.len, at.m, &per, &nqt);
+                    int64_t incl = tiles;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= o) incl += v;
+                    }
+                    const int64_t end = first + incl;
+                    unsigned todo = __ballot_sync(0xffffffffu,
+                                                  tiles > 0 && end > t0 && end - tiles < t1);
+                    while (ok && todo) {
+                        const int l = __ffs(todo) - 1;
+                        todo &= todo - 1;
+                        GroupAt o;
+                        o.l0 = __shfl_sync(0xffffffffu, at.l0, l);
+                        o.len = __shfl_sync(0xffffffffu, at.len, l);
+                        o.p0 = __shfl_sync(0xffffffffu, at.p0, l);
+                        o.m = __shfl_sync(0xffffffffu, at.m, l);
+                        const int64_t e = __shfl_sync(0xffffffffu, end, l);
+                        const int64_t b = e - __shfl_sync(0xffffffffu, tiles, l);
+                        queue_group(o, b, max(b, t0), min(e, t1));
+                    }
+                    first = __shfl_sync(0xffffffffu, end, 31);
+                }
+            }
+        } else {
+            queue_group(GroupAt{0, p.nx, 0, p.nq}, 0, t0, t1);
+        }
+        if (ok) queue(Item{0, 0, 0, 0, 0});
+    } else {
+        // ---- epilogue: warp w holds TMEM lanes 32 (w & 3) .. of the tile's rows
+        const int quarter = warp & 3, tid = threadIdx.x - kEpi0 * 32;
+        Item item;
+        for (int64_t i = 0;; ++i) {
+            // the four warps leave together: the barriers count them all
+            const bool got = next_item(i, &item);
+            if (named_bar_sync_or(kEpiBar, 128, !got)) break;
+            const int h = (int)(i & 1);
+            // where each column's scores go (tile i - 2's half of the table was read
+            // before every warp passed the barrier above for tile i - 1)
+            for (int c = tid; c < item.nq; c += 128) {
+                const int64_t pr = (int64_t)item.q0 + c;
+                int64_t at;
+                if constexpr (GROUP) {
+                    const int64_t row = p.g.pair_row ? (int64_t)p.g.pair_row[pr] : pr;
+                    at = p.g.out_off[pr];
+                    if (row < 0 || row >= p.nq || at < 0 ||
+                        at > p.g.out_n - (item.j0 + item.nx)) {
+                        if (row != -1) atomicOr(p.err + kScoreBadItem, 1);
+                        at = -1;
+                    } else {
+                        at += item.j0;
+                    }
+                } else {
+                    at = pr * p.ld_out + item.j0;
+                }
+                sm.base[h][c] = at;
+            }
+            const bool ok = mbar_wait(&sm.accfull[h], (uint32_t)(i >> 1) & 1u, &sm.abort);
+            if (named_bar_sync_or(kEpiBar + 1, 128, !ok)) break;
+            tc_fence_after();
+            const int row = quarter * 32 + lane;
+            const uint32_t acc =
+                tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(h * S::kAcc);
+            if (quarter * 32 < item.nx) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < item.nq; c0 += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(acc + (uint32_t)c0, r);
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        if (c0 + u >= item.nq) break;
+                        const int64_t at = sm.base[h][c0 + u];
+                        const float v = fmaf(p.alpha, __uint_as_float(r[u]), p.beta);
+                        if (at >= 0 && row < item.nx) {
+                            if constexpr (sizeof(O) == 4) out[at + row] = v;
+                            else out[at + row] = __float2bfloat16_rn(v);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.accempty[h]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && sm.abort) atomicOr(p.err + kScoreTimeout, 1);
+    if (warp == 0) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmem);
+    }
+}
+
+void row_map(CUtensorMap* m, const m3g_rows& r, int box_rows) {
+    const bool f8 = r.dtype == M3G_E4M3;
+    encode_tma_2d(m, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r.data,
+                  (uint64_t)r.dim, (uint64_t)r.n, (uint64_t)r.ld * (f8 ? 1 : 2),
+                  (uint32_t)(f8 ? kSlice : kSlice / 2), (uint32_t)box_rows,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <bool F8, int NT, bool GROUP, class O>
+cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* out,
+                   unsigned grid, cudaStream_t st) {
+    constexpr size_t smem = sizeof(Smem<NT>) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    auto kernel = scores_tc_kernel<F8, NT, GROUP, O>;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    CUtensorMap mx, mx32, mq;
+    row_map(&mx, x, kM);
+    row_map(&mx32, x, 32);
+    row_map(&mq, q, GROUP && p.g.pair_row ? 1 : Shape<NT>::kBox);
+    kernel<<<grid, kThreads, smem, st>>>(mx, mx32, mq, static_cast<O*>(out), p);
+    return cudaGetLastError();
+}
+
+template <bool GROUP>
+cudaError_t launch_any(const m3g_rows& q, const m3g_rows& x, const Params& p, bool wide, void* out,
+                       int out_dtype, unsigned grid, cudaStream_t st) {
+    const bool f32 = out_dtype == M3G_F32;
+    if (x.dtype == M3G_E4M3) {
+        if (wide)
+            return f32 ? launch<true, 240, GROUP, float>(q, x, p, out, grid, st)
+                       : launch<true, 240, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+        return f32 ? launch<true, 64, GROUP, float>(q, x, p, out, grid, st)
+                   : launch<true, 64, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+    }
+    if (wide)
+        return f32 ? launch<false, 240, GROUP, float>(q, x, p, out, grid, st)
+                   : launch<false, 240, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+    return f32 ? launch<false, 64, GROUP, float>(q, x, p, out, grid, st)
+               : launch<false, 64, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+}
+
+Params params_of(const m3g_rows& q, const m3g_rows& x, float alpha, float beta, int* err) {
+    Params p{};
+    p.nq = q.n;
+    p.nx = x.n;
+    p.row_bytes = x.dim * (x.dtype == M3G_E4M3 ? 1 : 2);
+    p.nk = (p.row_bytes + kSlice - 1) / kSlice;
+    p.qs = q.scales;
+    p.xs = x.scales;
+    p.lqs = q.ld_scales;
+    p.lxs = x.ld_scales;
+    p.alpha = alpha;
+    p.beta = beta;
+    p.err = err;
+    return p;
+}
+
+}  // namespace
+
+cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
+                              void* out, int out_dtype, int64_t ld_out, int* err, int sms,
+                              cudaStream_t st) {
+    Params p = params_of(q, x, alpha, beta, err);
+    p.ld_out = ld_out;
+    const bool wide = q.n > 64;
+    const int64_t tiles = (x.n + kM - 1) / kM * ((q.n + 15) / 16);  // at least as many as there are
+    return launch_any<false>(q, x, p, wide, out, out_dtype,
+                             (unsigned)std::min<int64_t>(tiles, sms), st);
+}
+
+cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const ScoreGroups& g,
+                               float alpha, float beta, void* out, int out_dtype, int* err,
+                               int sms, cudaStream_t st) {
+    Params p = params_of(q, x, alpha, beta, err);
+    p.g = g;
+    const bool wide = g.npair / g.ngroup > 64;
+    return launch_any<true>(q, x, p, wide, out, out_dtype, (unsigned)sms, st);
+}
+
+}  // namespace m3g

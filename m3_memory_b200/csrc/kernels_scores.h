@@ -1,4 +1,5 @@
-// kernels_scores.h -- launchers of the row-score kernels (k_scores.cu, k_probs.cu).
+// kernels_scores.h -- launchers of the row-score kernels (k_pack.cu, k_scores_tc.cu,
+// k_probs.cu).
 #pragma once
 
 #include <cuda_runtime.h>
