@@ -19,7 +19,7 @@
 // 128 rows, up to NT queries; queries fastest, so the rows come from L2 after their
 // first tile).  Warp 0 loads (TMA; queries of a group by gather4), warp 1 issues
 // the MMAs, warp 2 brings scale words, warp 3 walks the groups and queues tiles,
-// warps 4-7 store.  Every wait is bounded.
+// warps 4-11 store.  Every wait is bounded.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -36,10 +36,10 @@ namespace {
 constexpr int kM = 128;                 // rows of x a tile
 constexpr int kSlice = 128;             // bytes of a row a stage (128 8-bit or 64 bf16 dims)
 constexpr int kXBytes = kM * kSlice;
-constexpr int kThreads = 256;
+constexpr int kEpiWarps = 8;            // two for each quarter of the TMEM lanes
+constexpr int kThreads = (4 + kEpiWarps) * 32;
 constexpr int kEpi0 = 4;                // first epilogue warp
 constexpr int kItems = 4;               // tiles queued ahead
-constexpr int kEpiBar = 1;              // named barriers of the epilogue warps: this and the next
 
 // The two launch shapes: up to 64 queries a tile with eight stages in flight, for
 // rows that are read for a few queries each, and up to 240 with four.
@@ -62,16 +62,18 @@ struct Item {
 };
 
 constexpr int kSfBytes = 512 + 1024;  // scale words of a 512-dim chunk: x rows, queries
+constexpr int kSfSlots = 4;           // chunks of them in shared memory (two in TMEM)
 
 template <int NT>
 struct alignas(1024) Smem {
     unsigned char stage[Shape<NT>::kStages][kXBytes + NT * kSlice];
-    unsigned char sf[2][kSfBytes];
-    int64_t base[2][NT];  // where each column's scores start; -1: nowhere
+    unsigned char sf[kSfSlots][kSfBytes];
+    int64_t at[kItems][NT];  // where each column's scores start; -1: nowhere
+    alignas(16) int32_t row[kItems][NT];  // each column's row of q (0 where there is none)
     int64_t prefix[kThreads + 1];
     Item items[kItems];
     uint64_t full[Shape<NT>::kStages], empty[Shape<NT>::kStages];
-    uint64_t accfull[2], accempty[2], sffull[2], sfempty[2];
+    uint64_t accfull[2], accempty[2], sffull[kSfSlots], sfempty[kSfSlots];
     uint64_t itemfull[kItems], itemempty[kItems], drain;
     int64_t warp_sum[kThreads / 32];
     uint32_t tmem;
@@ -124,10 +126,25 @@ __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint32_t saddr) {
 // kind::mxf8f6f4: both operands e4m3 (0) and K-major, N >> 3 at bits 17-22, ue8m0
 // scales (bit 23), M >> 7 at bits 27-28; the scale byte of the words: bits 4-5 (B)
 // and 29-30 (A).
-__device__ __forceinline__ uint32_t mx_idesc(int n, int byte) {
-    return ((uint32_t)byte << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27) |
-           ((uint32_t)byte << 29);
+__device__ __forceinline__ uint32_t mx_idesc(int n) {
+    return ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27);
 }
+__device__ __forceinline__ uint32_t mx_idesc_byte(uint32_t idesc, int byte) {
+    return idesc | ((uint32_t)byte << 4) | ((uint32_t)byte << 29);
+}
+
+// A position in a ring of N slots and the parity of its current round.
+template <int N>
+struct Ring {
+    uint32_t i = 0, phase = 0, n = 0;
+    __device__ __forceinline__ void next() {
+        ++n;
+        if (++i == N) {
+            i = 0;
+            phase ^= 1u;
+        }
+    }
+};
 
 // A group's tiles: its rows in 128s times its pairs in nqt parts of `per`.
 template <int NT>
@@ -178,13 +195,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sm.accfull[s], 1);
-            mbar_init(&sm.accempty[s], 4);
+            mbar_init(&sm.accempty[s], kEpiWarps);
+        }
+        for (int s = 0; s < kSfSlots; ++s) {
             mbar_init(&sm.sffull[s], 1);
             mbar_init(&sm.sfempty[s], 1);
         }
         for (int s = 0; s < kItems; ++s) {
             mbar_init(&sm.itemfull[s], 1);
-            mbar_init(&sm.itemempty[s], F8 ? 7 : 6);  // warps 0, 1, (2,) 4-7
+            mbar_init(&sm.itemempty[s], kEpiWarps + (F8 ? 3 : 2));  // its readers' warps
         }
         mbar_init(&sm.drain, 1);
         sm.abort = 0;
@@ -237,182 +256,209 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t t1 = t0 + share + ((int64_t)blockIdx.x < more ? 1 : 0);
     const uint32_t tmem = sm.tmem;
 
-    // The next queued tile; false: none left, or the launch gave up.
+    // The next queued tile; false: none left, or the launch gave up.  done_with()
+    // hands its slot back.
     auto next_item = [&](int64_t i, Item* it) {
         const int s = (int)(i % kItems);
         const bool ok = mbar_wait(&sm.itemfull[s], (uint32_t)(i / kItems) & 1u, &sm.abort);
         if (ok) *it = sm.items[s];
         __syncwarp();
         if (!__all_sync(0xffffffffu, ok)) return false;
-        if (lane == 0) mbar_arrive(&sm.itemempty[s]);
         return it->nx > 0;
     };
+    auto done_with = [&](int64_t i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.itemempty[i % kItems]);
+    };
+    const bool gather = GROUP && p.g.pair_row != nullptr;
     auto columns = [](const Item& it) { return (it.nq + 15) & ~15; };
 
     if (warp == 0) {
-        // ---- loads
-        int64_t it = 0;
+        // ---- loads.  The whole warp walks the tiles with warp-uniform values, so the
+        // copies' operands stay in uniform registers; the elected lane issues.
+        const bool leader = elect_one();
+        Ring<S::kStages> ring;
         bool ok = true;
         Item item;
         for (int64_t i = 0; ok && next_item(i, &item); ++i) {
             const int n = columns(item);
-            int rows[2][4];  // the rows of gathers lane and lane + 32
-            uint32_t qbytes;
-            const bool gather = GROUP && p.g.pair_row != nullptr;
-            if (gather) {
-#pragma unroll
-                for (int h = 0; h < (NT > 128 ? 2 : 1); ++h)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int c = 4 * (lane + 32 * h) + u;
-                        const int r = c < item.nq ? p.g.pair_row[item.q0 + c] : 0;
-                        rows[h][u] = r >= 0 && r < p.nq ? r : 0;
-                    }
-                qbytes = (uint32_t)n * kSlice;
-            } else {
-                qbytes = (uint32_t)((n + S::kBox - 1) / S::kBox * S::kBox) * kSlice;
-            }
+            const int32_t* rows = sm.row[i % kItems];
+            const int qboxes = gather ? n / 4 : (n + S::kBox - 1) / S::kBox;
             const int xboxes = item.nx > 96 ? 0 : (item.nx + 31) / 32;
-            const uint32_t bytes = qbytes + (xboxes ? (uint32_t)xboxes * 32 * kSlice : kXBytes);
-            for (int kt = 0; kt < p.nk; ++kt, ++it) {
-                const int s = (int)(it % S::kStages);
-                if (it >= S::kStages)
-                    ok = mbar_wait(&sm.empty[s], (uint32_t)((it / S::kStages) - 1) & 1u,
-                                   &sm.abort);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                unsigned char* sx = sm.stage[s];
-                unsigned char* sq = sx + kXBytes;
-                const int x = kt * (F8 ? kSlice : kSlice / 2);
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&sm.full[s], bytes);
+            const uint32_t bytes = (uint32_t)kSlice * (qboxes * (gather ? 4 : S::kBox) +
+                                                       (xboxes ? xboxes * 32 : kM));
+            for (int kt = 0; kt < p.nk; ++kt) {
+                if (ring.n >= S::kStages &&
+                    !__all_sync(0xffffffffu,
+                                mbar_wait(&sm.empty[ring.i], ring.phase ^ 1u, &sm.abort))) {
+                    ok = false;
+                    break;
+                }
+                if (leader) {
+                    uint64_t* bar = &sm.full[ring.i];
+                    unsigned char* sx = sm.stage[ring.i];
+                    unsigned char* sq = sx + kXBytes;
+                    const int x = kt * (F8 ? kSlice : kSlice / 2);
+                    mbar_arrive_expect_tx(bar, bytes);
                     if (xboxes == 0) {
-                        tma_load_2d(sx, &map_x, x, item.x0, &sm.full[s]);
+                        tma_load_2d(sx, &map_x, x, item.x0, bar);
                     } else {
                         for (int b = 0; b < xboxes; ++b)
-                            tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b,
-                                        &sm.full[s]);
+                            tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b, bar);
                     }
-                    if (!gather)
-                        for (int b = 0; b * S::kBox < n; ++b)
+                    if (gather) {
+                        for (int b = 0; b < qboxes; ++b) {
+                            const int4 r = *reinterpret_cast<const int4*>(rows + 4 * b);
+                            tma_gather4(sq + b * 4 * kSlice, &map_q, x, r.x, r.y, r.z, r.w, bar);
+                        }
+                    } else {
+                        for (int b = 0; b < qboxes; ++b)
                             tma_load_2d(sq + b * S::kBox * kSlice, &map_q, x,
-                                        item.q0 + b * S::kBox, &sm.full[s]);
+                                        item.q0 + b * S::kBox, bar);
+                    }
                 }
                 __syncwarp();
-                if (gather) {
-#pragma unroll
-                    for (int h = 0; h < (NT > 128 ? 2 : 1); ++h) {
-                        const int c = 4 * (lane + 32 * h);
-                        if (c < n)
-                            tma_gather4(sq + c * kSlice, &map_q, x, rows[h][0], rows[h][1],
-                                        rows[h][2], rows[h][3], &sm.full[s]);
-                    }
-                }
+                ring.next();
             }
+            done_with(i);
         }
         // no copy may still be landing when the CTA leaves
-        if (lane == 0)
-            for (int64_t k = it > S::kStages ? it - S::kStages : 0; k < it; ++k)
-                mbar_drain(&sm.full[k % S::kStages], (uint32_t)(k / S::kStages) & 1u);
+        if (leader)
+            for (uint32_t k = ring.n > S::kStages ? ring.n - S::kStages : 0u; k < ring.n; ++k)
+                mbar_drain(&sm.full[k % S::kStages], (k / S::kStages) & 1u);
+        __syncwarp();
     } else if (warp == 1) {
-        // ---- MMAs: tile i accumulates in TMEM half i & 1
-        int64_t it = 0, sf = 0;
+        // ---- MMAs: tile i accumulates in TMEM half i & 1.  Warp-uniform like the loads.
+        const bool leader = elect_one();
+        // descriptors of the first stage; an offset of b bytes adds b >> 4
+        const uint64_t dx0 = sw128_desc(smem_u32(sm.stage[0]));
+        const uint64_t dq0 = sw128_desc(smem_u32(sm.stage[0]) + kXBytes);
+        constexpr uint64_t kStep = (kXBytes + NT * kSlice) >> 4;
+        Ring<S::kStages> ring;
+        Ring<kSfSlots> sf;
         bool ok = true;
         Item item;
         for (int64_t i = 0; ok && next_item(i, &item); ++i) {
             const int h = (int)(i & 1), n = columns(item);
-            if (i >= 2)
-                ok = mbar_wait(&sm.accempty[h], (uint32_t)((i >> 1) - 1) & 1u, &sm.abort);
+            done_with(i);
+            if (i >= 2 &&
+                !__all_sync(0xffffffffu, mbar_wait(&sm.accempty[h], (uint32_t)((i >> 1) - 1) & 1u,
+                                                   &sm.abort)))
+                break;
             tc_fence_after();
             const uint32_t d = tmem + (uint32_t)(h * S::kAcc);
-            for (int kt = 0; ok && kt < p.nk; ++kt, ++it) {
-                const int s = (int)(it % S::kStages);
-                const int c = (int)(sf & 1);
-                const uint32_t tsf = tmem + (uint32_t)(S::kSf0 + c * S::kSfStep);
-                if (F8 && (kt & 3) == 0)
-                    ok = mbar_wait(&sm.sffull[c], (uint32_t)(sf >> 1) & 1u, &sm.abort);
-                ok = ok && mbar_wait(&sm.full[s], (uint32_t)(it / S::kStages) & 1u, &sm.abort);
-                if (!ok) break;
+            const uint32_t idesc = F8 ? mx_idesc(n) : tc_idesc_m128(n, 1);
+            for (int kt = 0; kt < p.nk; ++kt) {
+                const bool first = F8 && (kt & 3) == 0;
+                const bool last = F8 && ((kt & 3) == 3 || kt + 1 == p.nk);
+                const uint32_t tsf = tmem + (uint32_t)(S::kSf0 + (int)(sf.n & 1u) * S::kSfStep);
+                bool go = true;
+                if (first) {
+                    // the chunk's words, and its place in TMEM (the chunk two before it)
+                    go = mbar_wait(&sm.sffull[sf.i], sf.phase, &sm.abort);
+                    if (go && sf.n >= 2)
+                        go = mbar_wait(&sm.sfempty[(sf.n - 2) % kSfSlots],
+                                       ((sf.n - 2) / kSfSlots) & 1u, &sm.abort);
+                }
+                go = go && mbar_wait(&sm.full[ring.i], ring.phase, &sm.abort);
+                if (!__all_sync(0xffffffffu, go)) {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
-                if (lane == 0) {
-                    if (F8 && (kt & 3) == 0) {
-                        const uint32_t src = smem_u32(sm.sf[c]);
+                if (leader) {
+                    if (first) {
+                        const uint32_t src = smem_u32(sm.sf[sf.i]);
                         tc_copy_scales(tsf, src);
                         tc_copy_scales(tsf + 4, src + 512);
                         if (NT > 128) tc_copy_scales(tsf + 8, src + 1024);
                     }
-                    const uint32_t sx = smem_u32(sm.stage[s]), sq = sx + kXBytes;
+                    const uint64_t a = dx0 + ring.i * kStep, b = dq0 + ring.i * kStep;
                     const int left = (p.row_bytes - kt * kSlice + 31) / 32;  // 32-byte steps
 #pragma unroll
                     for (int k = 0; k < kSlice / 32; ++k) {
                         if (k >= left) break;
-                        const uint64_t a = sw128_desc(sx + k * 32), b = sw128_desc(sq + k * 32);
                         if (F8)
-                            tc_mma_mx(d, a, b, mx_idesc(n, kt & 3), tsf, tsf + 4, (kt | k) != 0);
+                            tc_mma_mx(d, a + 2 * k, b + 2 * k, mx_idesc_byte(idesc, kt & 3), tsf,
+                                      tsf + 4, (kt | k) != 0);
                         else
-                            tc_mma_f16(d, a, b, tc_idesc_m128(n, 1), (kt | k) != 0);
+                            tc_mma_f16(d, a + 2 * k, b + 2 * k, idesc, (kt | k) != 0);
                     }
-                    tc_commit(&sm.empty[s]);
-                    if (F8 && ((kt & 3) == 3 || kt + 1 == p.nk)) tc_commit(&sm.sfempty[c]);
+                    tc_commit(&sm.empty[ring.i]);
+                    if (last) tc_commit(&sm.sfempty[sf.i]);
                     if (kt + 1 == p.nk) tc_commit(&sm.accfull[h]);
                 }
-                if (F8 && ((kt & 3) == 3 || kt + 1 == p.nk)) ++sf;
                 __syncwarp();
+                ring.next();
+                if (last) sf.next();
             }
-            ok = __all_sync(0xffffffffu, ok);
         }
-        if (lane == 0) {
+        if (leader) {
             // fires once every MMA issued above has completed (also on an error path)
             tc_commit(&sm.drain);
             mbar_drain(&sm.drain, 0);
         }
+        __syncwarp();
     } else if (warp == 2) {
         if constexpr (F8) {
-            // ---- scale words: lane r brings rows r, r + 32, ..; the slot of chunk c
-            // is free in shared memory and in TMEM once chunk c - 2's MMAs are done
-            int64_t sf = 0;
-            bool ok = true;
+            // ---- scale words, read one chunk ahead of the one being handed over:
+            // lane r brings rows r, r + 32, ..
+            constexpr int W = 4 + (NT > 128 ? 8 : 4);
+            const uint8_t* ptr[W];
+            uint32_t next[W];
             Item item;
-            for (int64_t i = 0; ok && next_item(i, &item); ++i) {
-                const uint8_t *xp[4], *qp[NT > 128 ? 8 : 4];
+            int64_t i = 0, sf = 0;
+            auto load = [&](int kt) {
+#pragma unroll
+                for (int u = 0; u < W; ++u)
+                    next[u] = ptr[u] ? __ldg(reinterpret_cast<const uint32_t*>(ptr[u] + kt))
+                                     : 0x7F7F7F7Fu;  // ones
+            };
+            auto open = [&] {
+                if (!next_item(i, &item)) return false;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int r = lane + 32 * u;
-                    xp[u] = r < item.nx ? p.xs + (item.x0 + r) * p.lxs : nullptr;
+                    ptr[u] = r < item.nx ? p.xs + (item.x0 + r) * p.lxs : nullptr;
                 }
 #pragma unroll
-                for (int u = 0; u < (NT > 128 ? 8 : 4); ++u) {
+                for (int u = 0; u < W - 4; ++u) {
                     const int c = lane + 32 * u;
-                    qp[u] = nullptr;
-                    if (c < item.nq) {
-                        int64_t r = (int64_t)item.q0 + c;
-                        if (GROUP && p.g.pair_row) r = p.g.pair_row[r];
-                        if (r >= 0 && r < p.nq) qp[u] = p.qs + r * p.lqs;
-                    }
+                    const int64_t r = gather ? (c < item.nq ? sm.row[i % kItems][c] : 0)
+                                             : (int64_t)item.q0 + c;
+                    ptr[4 + u] = c < item.nq ? p.qs + r * p.lqs : nullptr;
                 }
-                for (int kt = 0; kt < p.nk; kt += 4, ++sf) {
-                    const uint32_t one = 0x7F7F7F7Fu;
-                    uint32_t w[4 + (NT > 128 ? 8 : 4)];
+                done_with(i++);
+                load(0);
+                return true;
+            };
+            bool ok = open();
+            for (int kt = 0; ok; ++sf) {
+                uint32_t w[W];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        w[u] = xp[u] ? __ldg(reinterpret_cast<const uint32_t*>(xp[u] + kt)) : one;
-#pragma unroll
-                    for (int u = 0; u < (NT > 128 ? 8 : 4); ++u)
-                        w[4 + u] =
-                            qp[u] ? __ldg(reinterpret_cast<const uint32_t*>(qp[u] + kt)) : one;
-                    const int c = (int)(sf & 1);
-                    if (sf >= 2)
-                        ok = mbar_wait(&sm.sfempty[c], (uint32_t)((sf >> 1) - 1) & 1u, &sm.abort);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-#pragma unroll
-                    for (int u = 0; u < 4 + (NT > 128 ? 8 : 4); u += 4)
-                        *reinterpret_cast<uint4*>(sm.sf[c] + 128 * u + 16 * lane) =
-                            make_uint4(w[u], w[u + 1], w[u + 2], w[u + 3]);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.sffull[c]);
+                for (int u = 0; u < W; ++u) w[u] = next[u];
+                kt += 4;
+                bool more = true;
+                if (kt < p.nk) {
+                    load(kt);
+                } else {
+                    kt = 0;
+                    more = open();
                 }
+                const int c = (int)(sf % kSfSlots);
+                if (sf >= kSfSlots)
+                    ok = mbar_wait(&sm.sfempty[c], (uint32_t)((sf / kSfSlots) - 1) & 1u,
+                                   &sm.abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int u = 0; u < W; u += 4)
+                    *reinterpret_cast<uint4*>(sm.sf[c] + 128 * u + 16 * lane) =
+                        make_uint4(w[u], w[u + 1], w[u + 2], w[u + 3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.sffull[c]);
+                ok = more;
             }
         }
     } else if (warp == 3) {
@@ -425,6 +471,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = mbar_wait(&sm.itemempty[s], (uint32_t)((i / kItems) - 1) & 1u, &sm.abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
+            if constexpr (GROUP) {
+                for (int c = lane; c < columns(item); c += 32) {
+                    if (c >= item.nq) {
+                        sm.row[s][c] = 0;
+                        continue;
+                    }
+                    const int64_t pr = (int64_t)item.q0 + c;
+                    const int64_t row = gather ? (int64_t)p.g.pair_row[pr] : pr;
+                    const int64_t at = p.g.out_off[pr];
+                    const bool in = row >= 0 && row < p.nq && at >= 0 &&
+                                    at <= p.g.out_n - (item.j0 + item.nx);
+                    if (!in && row != -1) atomicOr(p.err + kScoreBadItem, 1);
+                    sm.row[s][c] = in ? (int32_t)row : 0;
+                    sm.at[s][c] = in ? at + item.j0 : -1;
+                }
+                __syncwarp();
+            }
             if (lane == 0) {
                 sm.items[s] = item;
                 mbar_arrive(&sm.itemfull[s]);
@@ -436,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // tiles from .. to - 1 of the launch, of the group whose first one is `first`
             int per, nqt;
             group_tiles<NT>(at.len, at.m, &per, &nqt);
-            for (int64_t t = from; ok && t < to; ++t) {
+            for (int64_t t = from; ok && t < to; t += GROUP ? 1 : gridDim.x) {
                 const int64_t xt = (t - first) / nqt, qt = (t - first) % nqt;
                 Item item;
                 item.j0 = xt * kM;
@@ -486,61 +549,51 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else {
-            queue_group(GroupAt{0, p.nx, 0, p.nq}, 0, t0, t1);
+            queue_group(GroupAt{0, p.nx, 0, p.nq}, 0, blockIdx.x, total);
         }
         if (ok) queue(Item{0, 0, 0, 0, 0});
     } else {
-        // ---- epilogue: warp w holds TMEM lanes 32 (w & 3) .. of the tile's rows
-        const int quarter = warp & 3, tid = threadIdx.x - kEpi0 * 32;
+        // ---- epilogue: warp w holds TMEM lanes 32 (w & 3) .. of the tile's rows, and
+        // every other 16 columns
+        const int quarter = warp & 3, half = (warp - kEpi0) >> 2;
+        const int row = quarter * 32 + lane;
         Item item;
-        for (int64_t i = 0;; ++i) {
-            // the four warps leave together: the barriers count them all
-            const bool got = next_item(i, &item);
-            if (named_bar_sync_or(kEpiBar, 128, !got)) break;
+        for (int64_t i = 0; next_item(i, &item); ++i) {
             const int h = (int)(i & 1);
-            // where each column's scores go (tile i - 2's half of the table was read
-            // before every warp passed the barrier above for tile i - 1)
-            for (int c = tid; c < item.nq; c += 128) {
-                const int64_t pr = (int64_t)item.q0 + c;
-                int64_t at;
-                if constexpr (GROUP) {
-                    const int64_t row = p.g.pair_row ? (int64_t)p.g.pair_row[pr] : pr;
-                    at = p.g.out_off[pr];
-                    if (row < 0 || row >= p.nq || at < 0 ||
-                        at > p.g.out_n - (item.j0 + item.nx)) {
-                        if (row != -1) atomicOr(p.err + kScoreBadItem, 1);
-                        at = -1;
-                    } else {
-                        at += item.j0;
-                    }
-                } else {
-                    at = pr * p.ld_out + item.j0;
-                }
-                sm.base[h][c] = at;
-            }
             const bool ok = mbar_wait(&sm.accfull[h], (uint32_t)(i >> 1) & 1u, &sm.abort);
-            if (named_bar_sync_or(kEpiBar + 1, 128, !ok)) break;
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            const int row = quarter * 32 + lane;
             const uint32_t acc =
                 tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(h * S::kAcc);
             if (quarter * 32 < item.nx) {
+                O* mine = out + row;
+                if constexpr (!GROUP) mine += (int64_t)item.q0 * p.ld_out + item.j0;
+                const bool in = row < item.nx;
 #pragma unroll 1
-                for (int c0 = 0; c0 < item.nq; c0 += 16) {
+                for (int c0 = 16 * half; c0 < item.nq; c0 += 32) {
                     uint32_t r[16];
                     tmem_ld16(acc + (uint32_t)c0, r);
-#pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        if (c0 + u >= item.nq) break;
-                        const int64_t at = sm.base[h][c0 + u];
+                    auto put = [&](int u) {
                         const float v = fmaf(p.alpha, __uint_as_float(r[u]), p.beta);
-                        if (at >= 0 && row < item.nx) {
-                            if constexpr (sizeof(O) == 4) out[at + row] = v;
-                            else out[at + row] = __float2bfloat16_rn(v);
+                        int64_t at;
+                        if constexpr (GROUP) at = sm.at[i % kItems][c0 + u];
+                        else at = (c0 + u) * p.ld_out;
+                        if (in && (!GROUP || at >= 0)) {
+                            if constexpr (sizeof(O) == 4) mine[at] = v;
+                            else mine[at] = __float2bfloat16_rn(v);
                         }
+                    };
+                    if (c0 + 16 <= item.nq) {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) put(u);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u)
+                            if (c0 + u < item.nq) put(u);
                     }
                 }
             }
+            done_with(i);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.accempty[h]);
