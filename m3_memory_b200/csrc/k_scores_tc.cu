@@ -17,9 +17,9 @@
 //
 // A launch is one CTA per SM, each with an equal run of consecutive tiles (group,
 // 128 rows, up to NT queries; queries fastest, so the rows come from L2 after their
-// first tile).  Warp 0 loads (TMA; queries of a group by gather4), warp 1 issues
-// the MMAs, warp 2 brings scale words, warp 3 walks the groups and queues tiles,
-// warps 4-11 store.  Every wait is bounded.
+// first tile).  Warp 0 loads rows and warp 12 queries (TMA; those of a group by
+// gather4), warp 1 issues the MMAs, warp 2 brings scale words, warp 3 walks the
+// groups and queues tiles, warps 4-11 store.  Every wait is bounded.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -37,8 +37,8 @@ constexpr int kM = 128;                 // rows of x a tile
 constexpr int kSlice = 128;             // bytes of a row a stage (128 8-bit or 64 bf16 dims)
 constexpr int kXBytes = kM * kSlice;
 constexpr int kEpiWarps = 8;            // two for each quarter of the TMEM lanes
-constexpr int kThreads = (4 + kEpiWarps) * 32;
-constexpr int kEpi0 = 4;                // first epilogue warp
+constexpr int kThreads = (5 + kEpiWarps) * 32;
+constexpr int kEpi0 = 4;                // first epilogue warp (a multiple of 4)
 constexpr int kItems = 4;               // tiles queued ahead
 
 // The two launch shapes: up to 64 queries a tile with eight stages in flight, for
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) tmem_alloc(&sm.tmem, S::kTmem);
     if (threadIdx.x == 32) {
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.full[s], 2);  // the rows' and the queries' warps
             mbar_init(&sm.empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < kItems; ++s) {
             mbar_init(&sm.itemfull[s], 1);
-            mbar_init(&sm.itemempty[s], kEpiWarps + (F8 ? 3 : 2));  // its readers' warps
+            mbar_init(&sm.itemempty[s], kEpiWarps + (F8 ? 4 : 3));  // its readers' warps
         }
         mbar_init(&sm.drain, 1);
         sm.abort = 0;
@@ -273,10 +273,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool gather = GROUP && p.g.pair_row != nullptr;
     auto columns = [](const Item& it) { return (it.nq + 15) & ~15; };
 
-    if (warp == 0) {
-        // ---- loads.  The whole warp walks the tiles with warp-uniform values, so the
-        // copies' operands stay in uniform registers; the elected lane issues.
-        const bool leader = elect_one();
+    if (warp == 0 || warp == kThreads / 32 - 1) {
+        // ---- loads: warp 0 the rows, the last warp the queries (a copy takes its
+        // issuer some 100 cycles, and a stage has up to four of rows and sixty of
+        // gathered queries).  The warp walks the tiles with warp-uniform values, so
+        // the copies' operands stay in uniform registers; the elected lane issues.
+        const bool leader = elect_one(), xside = warp == 0;
         Ring<S::kStages> ring;
         bool ok = true;
         Item item;
@@ -285,8 +287,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int32_t* rows = sm.row[i % kItems];
             const int qboxes = gather ? n / 4 : (n + S::kBox - 1) / S::kBox;
             const int xboxes = item.nx > 96 ? 0 : (item.nx + 31) / 32;
-            const uint32_t bytes = (uint32_t)kSlice * (qboxes * (gather ? 4 : S::kBox) +
-                                                       (xboxes ? xboxes * 32 : kM));
+            const uint32_t bytes =
+                (uint32_t)kSlice * (xside ? (xboxes ? xboxes * 32 : kM)
+                                          : qboxes * (gather ? 4 : S::kBox));
             for (int kt = 0; kt < p.nk; ++kt) {
                 if (ring.n >= S::kStages &&
                     !__all_sync(0xffffffffu,
@@ -300,13 +303,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     unsigned char* sq = sx + kXBytes;
                     const int x = kt * (F8 ? kSlice : kSlice / 2);
                     mbar_arrive_expect_tx(bar, bytes);
-                    if (xboxes == 0) {
-                        tma_load_2d(sx, &map_x, x, item.x0, bar);
-                    } else {
-                        for (int b = 0; b < xboxes; ++b)
-                            tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b, bar);
-                    }
-                    if (gather) {
+                    if (xside) {
+                        if (xboxes == 0) {
+                            tma_load_2d(sx, &map_x, x, item.x0, bar);
+                        } else {
+                            for (int b = 0; b < xboxes; ++b)
+                                tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b,
+                                            bar);
+                        }
+                    } else if (gather) {
                         for (int b = 0; b < qboxes; ++b) {
                             const int4 r = *reinterpret_cast<const int4*>(rows + 4 * b);
                             tma_gather4(sq + b * 4 * kSlice, &map_q, x, r.x, r.y, r.z, r.w, bar);
@@ -322,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             done_with(i);
         }
-        // no copy may still be landing when the CTA leaves
+        // no copy may still be landing when the CTA leaves (where the other warp gave
+        // up first, the stage never fills and the wait ends at its limit)
         if (leader)
             for (uint32_t k = ring.n > S::kStages ? ring.n - S::kStages : 0u; k < ring.n; ++k)
                 mbar_drain(&sm.full[k % S::kStages], (k / S::kStages) & 1u);
