@@ -17,8 +17,8 @@
 //
 // A launch is one CTA per SM, each with an equal run of consecutive tiles (group,
 // 128 rows, up to NT queries; queries fastest, so the rows come from L2 after their
-// first tile).  Warp 0 loads rows and warp 12 queries (TMA; those of a group by
-// gather4), warp 1 issues the MMAs, warp 2 brings scale words, warp 3 walks the
+// first tile).  Warp 0 loads rows and warp 12 queries (TMA; those of a group
+// are gathered by warps 12-15), warp 1 issues the MMAs, warp 2 brings scale words, warp 3 walks the
 // groups and queues tiles, warps 4-11 store.  Every wait is bounded.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -37,9 +37,11 @@ constexpr int kM = 128;                 // rows of x a tile
 constexpr int kSlice = 128;             // bytes of a row a stage (128 8-bit or 64 bf16 dims)
 constexpr int kXBytes = kM * kSlice;
 constexpr int kEpiWarps = 8;            // two for each quarter of the TMEM lanes
-constexpr int kThreads = (5 + kEpiWarps) * 32;
+constexpr int kQueryWarps = 4;          // each gathers every fourth stage's queries
+constexpr int kThreads = (4 + kEpiWarps + kQueryWarps) * 32;
 constexpr int kEpi0 = 4;                // first epilogue warp (a multiple of 4)
-constexpr int kItems = 4;               // tiles queued ahead
+constexpr int kQuery0 = kEpi0 + kEpiWarps;
+constexpr int kItems = 8;               // tiles queued ahead
 
 // The two launch shapes: up to 64 queries a tile with eight stages in flight, for
 // rows that are read for a few queries each, and up to 240 with four.
@@ -84,6 +86,8 @@ struct Params {
     int64_t nq, nx;  // rows of q and x
     int nk;          // slices of a row
     int row_bytes;   // bytes of a row that hold dims
+    const void* q;
+    int64_t ldq;  // bytes
     const uint8_t *qs, *xs;
     int64_t lqs, lxs;
     float alpha, beta;
@@ -92,13 +96,13 @@ struct Params {
     int* err;
 };
 
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, int r0,
-                                            int r1, int r2, int r3, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
-        : "memory");
+// 16 bytes global -> shared, those past the first `size` filled with zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 __device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -203,7 +207,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < kItems; ++s) {
             mbar_init(&sm.itemfull[s], 1);
-            mbar_init(&sm.itemempty[s], kEpiWarps + (F8 ? 4 : 3));  // its readers' warps
+            // its readers' warps: rows, MMAs, scales, epilogue, queries
+            mbar_init(&sm.itemempty[s], 2 + (F8 ? 1 : 0) + kEpiWarps +
+                                            (GROUP && p.g.pair_row ? kQueryWarps : 1));
         }
         mbar_init(&sm.drain, 1);
         sm.abort = 0;
@@ -273,23 +279,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool gather = GROUP && p.g.pair_row != nullptr;
     auto columns = [](const Item& it) { return (it.nq + 15) & ~15; };
 
-    if (warp == 0 || warp == kThreads / 32 - 1) {
-        // ---- loads: warp 0 the rows, the last warp the queries (a copy takes its
-        // issuer some 100 cycles, and a stage has up to four of rows and sixty of
-        // gathered queries).  The warp walks the tiles with warp-uniform values, so
-        // the copies' operands stay in uniform registers; the elected lane issues.
-        const bool leader = elect_one(), xside = warp == 0;
+    if (warp >= kQuery0 && gather) {
+        // ---- a group's queries, gathered with 16-byte copies (TMA's gather4 takes
+        // some 230 cycles for its four rows): eight lanes a row, four rows a copy, in
+        // the 128-byte swizzle the MMA reads.  The copies are made visible to the
+        // tensor core by a fence that waits for all of the warp's, so each warp has
+        // one stage in flight and the warps take the stages in turn.
+        const unsigned char* src = static_cast<const unsigned char*>(p.q) + 16 * (lane & 7);
         Ring<S::kStages> ring;
         bool ok = true;
         Item item;
         for (int64_t i = 0; ok && next_item(i, &item); ++i) {
             const int n = columns(item);
             const int32_t* rows = sm.row[i % kItems];
-            const int qboxes = gather ? n / 4 : (n + S::kBox - 1) / S::kBox;
+            for (int kt = 0; kt < p.nk; ++kt, ring.next()) {
+                if (ring.n % kQueryWarps != (uint32_t)(warp - kQuery0)) continue;
+                if (ring.n >= S::kStages &&
+                    !__all_sync(0xffffffffu,
+                                mbar_wait(&sm.empty[ring.i], ring.phase ^ 1u, &sm.abort))) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = smem_u32(sm.stage[ring.i]) + kXBytes;
+                const int off = kt * kSlice;
+                const int left = p.row_bytes - off - 16 * (lane & 7);
+                const uint32_t size = left >= 16 ? 16u : left > 0 ? (uint32_t)left : 0u;
+                // (a copy of no bytes fills zeros; it is given an address in the row)
+                const unsigned char* at = src + (size ? off : -16 * (lane & 7));
+#pragma unroll 4
+                for (int r = lane >> 3; r < n; r += 4)
+                    cp_async16(dst + (uint32_t)(r * kSlice) + (((lane & 7) ^ (r & 7)) << 4),
+                               at + rows[r] * p.ldq, size);
+                cp_async_wait_all();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.full[ring.i]);
+            }
+            done_with(i);
+        }
+    } else if (warp == 0 || warp == kQuery0) {
+        // ---- loads by TMA: warp 0 the rows, the other the queries (a copy takes
+        // its issuer some 100 cycles).  The warp walks the tiles with warp-uniform
+        // values, so the copies' operands stay in uniform registers; the elected lane
+        // issues.
+        const bool leader = elect_one(), xside = warp == 0;
+        Ring<S::kStages> ring;
+        bool ok = true;
+        Item item;
+        for (int64_t i = 0; ok && next_item(i, &item); ++i) {
+            const int qboxes = (columns(item) + S::kBox - 1) / S::kBox;
             const int xboxes = item.nx > 96 ? 0 : (item.nx + 31) / 32;
             const uint32_t bytes =
-                (uint32_t)kSlice * (xside ? (xboxes ? xboxes * 32 : kM)
-                                          : qboxes * (gather ? 4 : S::kBox));
+                (uint32_t)kSlice * (xside ? (xboxes ? xboxes * 32 : kM) : qboxes * S::kBox);
+            done_with(i);
             for (int kt = 0; kt < p.nk; ++kt) {
                 if (ring.n >= S::kStages &&
                     !__all_sync(0xffffffffu,
@@ -303,29 +345,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     unsigned char* sq = sx + kXBytes;
                     const int x = kt * (F8 ? kSlice : kSlice / 2);
                     mbar_arrive_expect_tx(bar, bytes);
-                    if (xside) {
-                        if (xboxes == 0) {
-                            tma_load_2d(sx, &map_x, x, item.x0, bar);
-                        } else {
-                            for (int b = 0; b < xboxes; ++b)
-                                tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b,
-                                            bar);
-                        }
-                    } else if (gather) {
-                        for (int b = 0; b < qboxes; ++b) {
-                            const int4 r = *reinterpret_cast<const int4*>(rows + 4 * b);
-                            tma_gather4(sq + b * 4 * kSlice, &map_q, x, r.x, r.y, r.z, r.w, bar);
-                        }
-                    } else {
+                    if (!xside) {
                         for (int b = 0; b < qboxes; ++b)
                             tma_load_2d(sq + b * S::kBox * kSlice, &map_q, x,
                                         item.q0 + b * S::kBox, bar);
+                    } else if (xboxes == 0) {
+                        tma_load_2d(sx, &map_x, x, item.x0, bar);
+                    } else {
+                        for (int b = 0; b < xboxes; ++b)
+                            tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b, bar);
                     }
                 }
                 __syncwarp();
                 ring.next();
             }
-            done_with(i);
         }
         // no copy may still be landing when the CTA leaves (where the other warp gave
         // up first, the stage never fills and the wait ends at its limit)
@@ -635,7 +668,7 @@ cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* 
     CUtensorMap mx, mx32, mq;
     row_map(&mx, x, kM);
     row_map(&mx32, x, 32);
-    row_map(&mq, q, GROUP && p.g.pair_row ? 1 : Shape<NT>::kBox);
+    row_map(&mq, q, Shape<NT>::kBox);
     kernel<<<grid, kThreads, smem, st>>>(mx, mx32, mq, static_cast<O*>(out), p);
     return cudaGetLastError();
 }
@@ -664,6 +697,8 @@ Params params_of(const m3g_rows& q, const m3g_rows& x, float alpha, float beta, 
     p.nx = x.n;
     p.row_bytes = x.dim * (x.dtype == M3G_E4M3 ? 1 : 2);
     p.nk = (p.row_bytes + kSlice - 1) / kSlice;
+    p.q = q.data;
+    p.ldq = q.ld * (q.dtype == M3G_E4M3 ? 1 : 2);
     p.qs = q.scales;
     p.xs = x.scales;
     p.lqs = q.ld_scales;
