@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             queue_group(GroupAt{0, p.nx, 0, p.nq}, 0, blockIdx.x, total);
         }
         if (ok) queue(Item{0, 0, 0, 0, 0});
-    } else {
+    } else if (warp < kQuery0) {
         // ---- epilogue: warp w holds TMEM lanes 32 (w & 3) .. of the tile's rows, and
         // every other 16 columns
         const int quarter = warp & 3, half = (warp - kEpi0) >> 2;

@@ -160,7 +160,7 @@ def scores_ref(q, x, alpha, beta, out_dtype, dim):
 SHAPES = [(1, 1, 1), (1, 2, 128), (1, 300, 128), (1, 5000, 1024), (2, 127, 16), (3, 129, 100),
           (8, 1000, 256), (16, 128, 513), (17, 1000, 1024), (33, 257, 130), (64, 640, 768),
           (65, 333, 384), (129, 200, 90), (240, 256, 128), (241, 384, 256), (250, 513, 768),
-          (300, 700, 136), (700, 1300, 640), (1000, 129, 1100), (31, 40000, 64)]
+          (300, 700, 136), (700, 1300, 640), (1000, 129, 1100), (31, 40000, 64), (520, 60000, 64), (60, 200000, 32)]
 
 
 @pytest.mark.parametrize("nq,n,dim", SHAPES)
