@@ -15,9 +15,8 @@
 // slices of a 512-dim chunk take bytes 0..3 of the same TMEM words.  bf16 rows use
 // kind::f16.  Sums are fp32 in TMEM.
 //
-// A launch is one CTA per SM, each with an equal run of consecutive tiles (group,
-// 128 rows, up to NT queries; queries fastest, so the rows come from L2 after their
-// first tile).  Warp 0 loads rows and warp 12 queries (TMA; those of a group
+// A launch is one CTA per SM.  A tile is 128 rows of a group and up to NT of its
+// queries, queries fastest, so the rows come from L2 after their first tile.  Warp 0 loads rows and warp 12 queries (TMA; those of a group
 // are gathered by warps 12-15), warp 1 issues the MMAs, warp 2 brings scale words, warp 3 walks the
 // groups and queues tiles, warps 4-11 store.  Every wait is bounded.
 #include <cuda_bf16.h>
@@ -34,7 +33,7 @@ namespace m3g {
 namespace {
 
 constexpr int kM = 128;                 // rows of x a tile
-constexpr int kSlice = 128;             // bytes of a row a stage (128 8-bit or 64 bf16 dims)
+constexpr int kSlice = 128;             // bytes of a row a swizzled tile holds (128 8-bit or 64 bf16 dims)
 constexpr int kXBytes = kM * kSlice;
 constexpr int kEpiWarps = 8;            // two for each quarter of the TMEM lanes
 constexpr int kQueryWarps = 4;          // each gathers every fourth stage's queries
@@ -43,17 +42,19 @@ constexpr int kEpi0 = 4;                // first epilogue warp (a multiple of 4)
 constexpr int kQuery0 = kEpi0 + kEpiWarps;
 constexpr int kItems = 8;               // tiles queued ahead
 
-// The two launch shapes: up to 64 queries a tile with eight stages in flight, for
-// rows that are read for a few queries each, and up to 240 with four.
+// The two launch shapes: up to 64 queries a tile, for rows that are read for a few
+// queries each, with two slices a stage (a stage costs the MMA warp some 400 cycles
+// beside its MMAs), and up to 240 with one.
 template <int NT>
 struct Shape;
 template <>
 struct Shape<64> {
-    static constexpr int kStages = 8, kBox = 16, kAcc = 64, kTmem = 256, kSf0 = 128, kSfStep = 16;
+    static constexpr int kStages = 4, kSlices = 2, kBox = 16, kAcc = 64, kTmem = 256, kSf0 = 128,
+                         kSfStep = 16;
 };
 template <>
 struct Shape<240> {  // each accumulator's scales in the 16 columns behind it
-    static constexpr int kStages = 4, kBox = 48, kAcc = 256, kTmem = 512, kSf0 = 240,
+    static constexpr int kStages = 4, kSlices = 1, kBox = 48, kAcc = 256, kTmem = 512, kSf0 = 240,
                          kSfStep = 256;
 };
 
@@ -68,7 +69,7 @@ constexpr int kSfSlots = 4;           // chunks of them in shared memory (two in
 
 template <int NT>
 struct alignas(1024) Smem {
-    unsigned char stage[Shape<NT>::kStages][kXBytes + NT * kSlice];
+    unsigned char stage[Shape<NT>::kStages][Shape<NT>::kSlices][kXBytes + NT * kSlice];
     unsigned char sf[kSfSlots][kSfBytes];
     int64_t at[kItems][NT];  // where each column's scores start; -1: nowhere
     alignas(16) int32_t row[kItems][NT];  // each column's row of q (0 where there is none)
@@ -98,7 +99,7 @@ struct Params {
 
 // 16 bytes global -> shared, those past the first `size` filled with zeros.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
                  : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() {
@@ -150,17 +151,40 @@ struct Ring {
     }
 };
 
-// A group's tiles: its rows in 128s times its pairs in nqt parts of `per`.
+// A group's tiles: its rows in 128s (nx) times its pairs in nqt parts of `per`, the
+// pairs fastest.  CTAs take runs of equal weight: a tile of 32 b rows weighs 1 + 2 b
+// with few queries, where loading it is most of its time, and the same always with
+// many, where the MMAs are.
 template <int NT>
-__device__ __forceinline__ int64_t group_tiles(int64_t len, int64_t m, int* per, int* nqt) {
-    *per = NT;
-    *nqt = 0;
-    if (len <= 0 || m <= 0) return 0;
-    const int64_t parts = (m + NT - 1) / NT;
-    *per = (int)((((m + parts - 1) / parts) + 15) / 16 * 16);
-    *nqt = (int)((m + *per - 1) / *per);
-    return (len + kM - 1) / kM * *nqt;
-}
+struct Tiles {
+    int64_t nx;
+    int32_t per, nqt;
+    int32_t w, wlast;  // weight of a tile of 128 rows, and of the last rows' tiles
+
+    __device__ __forceinline__ Tiles(int64_t len, int64_t m) {
+        nx = len > 0 && m > 0 ? (len + kM - 1) / kM : 0;
+        uint32_t n = (uint32_t)m;  // pairs number less than 2^31
+        if (n > (uint32_t)NT) {
+            const uint32_t parts = (n + NT - 1) / NT;
+            n = (n + parts - 1) / parts;
+        }
+        per = (int32_t)max((n + 15u) & ~15u, 16u);
+        nqt = n == (uint32_t)m ? 1 : (int32_t)(((uint32_t)m + per - 1) / (uint32_t)per);
+        w = NT > 128 ? 1 : 9;
+        wlast = NT > 128 ? 1 : 1 + 2 * ((int32_t)(len - (nx - 1) * kM) + 31) / 32;
+    }
+    __device__ __forceinline__ int64_t count() const { return nx * nqt; }
+    __device__ __forceinline__ int64_t weight() const {
+        return nx > 0 ? ((nx - 1) * w + wlast) * nqt : 0;
+    }
+    // The first tile that starts at or after `at` (a weight from the group's start).
+    __device__ __forceinline__ int64_t first(int64_t at) const {
+        if (at <= 0) return 0;
+        if (at >= weight()) return count();
+        const int64_t whole = (nx - 1) * nqt, last = at - whole * w;
+        return last <= 0 ? (at + w - 1) / w : whole + (last + wlast - 1) / wlast;
+    }
+};
 
 // The group's rows and pairs; false (and nothing in it) when they are out of range.
 struct GroupAt {
@@ -221,8 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&map_q);
     }
 
-    // This CTA's run of tiles.  Grouped: the tiles of all groups are counted first,
-    // each thread a run of groups.
+    // This CTA's tiles.  Grouped: a run of the launch's weight, which is added up first,
+    // each thread a run of groups.  Dense: every gridDim.x-th tile.
     int64_t total;
     int64_t chunk = 0;  // groups a thread counts
     if constexpr (GROUP) {
@@ -230,11 +254,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t g0 = chunk * threadIdx.x, g1 = min(g0 + chunk, p.g.ngroup);
         int64_t mine = 0;
         bool ok = true;
+#pragma unroll 4
         for (int64_t i = g0; i < g1; ++i) {
             GroupAt at;
-            int per, nqt;
             ok &= load_group(p, i, &at);
-            mine += group_tiles<NT>(at.len, at.m, &per, &nqt);
+            mine += Tiles<NT>(at.len, at.m).weight();
         }
         if (!ok && blockIdx.x == 0) atomicOr(p.err + kScoreBadItem, 1);
         int64_t incl = mine;
@@ -250,16 +274,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         sm.prefix[threadIdx.x] = before + incl - mine;
         if (threadIdx.x == kThreads - 1) sm.prefix[kThreads] = before + incl;
     } else {
-        int per, nqt;
-        total = group_tiles<NT>(p.nx, p.nq, &per, &nqt);
+        total = Tiles<NT>(p.nx, p.nq).count();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if constexpr (GROUP) total = sm.prefix[kThreads];
-    const int64_t share = total / gridDim.x, more = total % gridDim.x;
-    const int64_t t0 = share * blockIdx.x + min((int64_t)blockIdx.x, more);
-    const int64_t t1 = t0 + share + ((int64_t)blockIdx.x < more ? 1 : 0);
+    const int64_t t0 = total / gridDim.x * blockIdx.x +
+                       total % gridDim.x * blockIdx.x / gridDim.x;
+    const int64_t t1 = total / gridDim.x * (blockIdx.x + 1) +
+                       total % gridDim.x * (blockIdx.x + 1) / gridDim.x;
     const uint32_t tmem = sm.tmem;
 
     // The next queued tile; false: none left, or the launch gave up.  done_with()
@@ -292,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int64_t i = 0; ok && next_item(i, &item); ++i) {
             const int n = columns(item);
             const int32_t* rows = sm.row[i % kItems];
-            for (int kt = 0; kt < p.nk; ++kt, ring.next()) {
+            for (int kt = 0; kt < p.nk; kt += S::kSlices, ring.next()) {
                 if (ring.n % kQueryWarps != (uint32_t)(warp - kQuery0)) continue;
                 if (ring.n >= S::kStages &&
                     !__all_sync(0xffffffffu,
@@ -300,16 +324,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ok = false;
                     break;
                 }
-                const uint32_t dst = smem_u32(sm.stage[ring.i]) + kXBytes;
-                const int off = kt * kSlice;
-                const int left = p.row_bytes - off - 16 * (lane & 7);
-                const uint32_t size = left >= 16 ? 16u : left > 0 ? (uint32_t)left : 0u;
-                // (a copy of no bytes fills zeros; it is given an address in the row)
-                const unsigned char* at = src + (size ? off : -16 * (lane & 7));
+#pragma unroll
+                for (int s = 0; s < S::kSlices; ++s) {
+                    if (kt + s >= p.nk) break;
+                    const uint32_t dst = smem_u32(sm.stage[ring.i][s]) + kXBytes;
+                    const int off = (kt + s) * kSlice;
+                    const int left = p.row_bytes - off - 16 * (lane & 7);
+                    const uint32_t size = left >= 16 ? 16u : left > 0 ? (uint32_t)left : 0u;
+                    // (a copy of no bytes fills zeros; it is given an address in the row)
+                    const unsigned char* at = src + (size ? off : -16 * (lane & 7));
 #pragma unroll 4
-                for (int r = lane >> 3; r < n; r += 4)
-                    cp_async16(dst + (uint32_t)(r * kSlice) + (((lane & 7) ^ (r & 7)) << 4),
-                               at + rows[r] * p.ldq, size);
+                    for (int r = lane >> 3; r < n; r += 4)
+                        cp_async16(dst + (uint32_t)(r * kSlice) + (((lane & 7) ^ (r & 7)) << 4),
+                                   at + rows[r] * p.ldq, size);
+                }
                 cp_async_wait_all();
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -332,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t bytes =
                 (uint32_t)kSlice * (xside ? (xboxes ? xboxes * 32 : kM) : qboxes * S::kBox);
             done_with(i);
-            for (int kt = 0; kt < p.nk; ++kt) {
+            for (int kt = 0; kt < p.nk; kt += S::kSlices) {
                 if (ring.n >= S::kStages &&
                     !__all_sync(0xffffffffu,
                                 mbar_wait(&sm.empty[ring.i], ring.phase ^ 1u, &sm.abort))) {
@@ -341,19 +369,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (leader) {
                     uint64_t* bar = &sm.full[ring.i];
-                    unsigned char* sx = sm.stage[ring.i];
-                    unsigned char* sq = sx + kXBytes;
-                    const int x = kt * (F8 ? kSlice : kSlice / 2);
-                    mbar_arrive_expect_tx(bar, bytes);
-                    if (!xside) {
-                        for (int b = 0; b < qboxes; ++b)
-                            tma_load_2d(sq + b * S::kBox * kSlice, &map_q, x,
-                                        item.q0 + b * S::kBox, bar);
-                    } else if (xboxes == 0) {
-                        tma_load_2d(sx, &map_x, x, item.x0, bar);
-                    } else {
-                        for (int b = 0; b < xboxes; ++b)
-                            tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b, bar);
+                    const int ns = min(S::kSlices, p.nk - kt);
+                    mbar_arrive_expect_tx(bar, bytes * ns);
+                    for (int s = 0; s < ns; ++s) {
+                        unsigned char* sx = sm.stage[ring.i][s];
+                        unsigned char* sq = sx + kXBytes;
+                        const int x = (kt + s) * (F8 ? kSlice : kSlice / 2);
+                        if (!xside) {
+                            for (int b = 0; b < qboxes; ++b)
+                                tma_load_2d(sq + b * S::kBox * kSlice, &map_q, x,
+                                            item.q0 + b * S::kBox, bar);
+                        } else if (xboxes == 0) {
+                            tma_load_2d(sx, &map_x, x, item.x0, bar);
+                        } else {
+                            for (int b = 0; b < xboxes; ++b)
+                                tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b,
+                                            bar);
+                        }
                     }
                 }
                 __syncwarp();
@@ -370,9 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- MMAs: tile i accumulates in TMEM half i & 1.  Warp-uniform like the loads.
         const bool leader = elect_one();
         // descriptors of the first stage; an offset of b bytes adds b >> 4
-        const uint64_t dx0 = sw128_desc(smem_u32(sm.stage[0]));
-        const uint64_t dq0 = sw128_desc(smem_u32(sm.stage[0]) + kXBytes);
-        constexpr uint64_t kStep = (kXBytes + NT * kSlice) >> 4;
+        const uint64_t dx0 = sw128_desc(smem_u32(sm.stage[0][0]));
+        constexpr uint32_t kStep = (kXBytes + NT * kSlice) >> 4;  // a slice
         Ring<S::kStages> ring;
         Ring<kSfSlots> sf;
         bool ok = true;
@@ -387,9 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t d = tmem + (uint32_t)(h * S::kAcc);
             const uint32_t idesc = F8 ? mx_idesc(n) : tc_idesc_m128(n, 1);
-            for (int kt = 0; kt < p.nk; ++kt) {
+            for (int kt = 0; kt < p.nk; kt += S::kSlices) {
                 const bool first = F8 && (kt & 3) == 0;
-                const bool last = F8 && ((kt & 3) == 3 || kt + 1 == p.nk);
+                const bool end = kt + S::kSlices >= p.nk;
+                const bool last = F8 && (((kt + S::kSlices) & 3) == 0 || end);
                 const uint32_t tsf = tmem + (uint32_t)(S::kSf0 + (int)(sf.n & 1u) * S::kSfStep);
                 bool go = true;
                 if (first) {
@@ -412,20 +444,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc_copy_scales(tsf + 4, src + 512);
                         if (NT > 128) tc_copy_scales(tsf + 8, src + 1024);
                     }
-                    const uint64_t a = dx0 + ring.i * kStep, b = dq0 + ring.i * kStep;
-                    const int left = (p.row_bytes - kt * kSlice + 31) / 32;  // 32-byte steps
+                    auto mma = [&](int s, int k, uint32_t id) {
+                        const uint64_t a = dx0 + (ring.i * S::kSlices + s) * kStep + 2 * k;
+                        const uint64_t b = a + (kXBytes >> 4);
+                        if (F8) tc_mma_mx(d, a, b, id, tsf, tsf + 4, (kt | s | k) != 0);
+                        else tc_mma_f16(d, a, b, id, (kt | s | k) != 0);
+                    };
 #pragma unroll
-                    for (int k = 0; k < kSlice / 32; ++k) {
-                        if (k >= left) break;
-                        if (F8)
-                            tc_mma_mx(d, a + 2 * k, b + 2 * k, mx_idesc_byte(idesc, kt & 3), tsf,
-                                      tsf + 4, (kt | k) != 0);
-                        else
-                            tc_mma_f16(d, a + 2 * k, b + 2 * k, idesc, (kt | k) != 0);
+                    for (int s = 0; s < S::kSlices; ++s) {
+                        const int left = p.row_bytes - (kt + s) * kSlice;  // bytes
+                        const uint32_t id = F8 ? mx_idesc_byte(idesc, (kt + s) & 3) : idesc;
+                        if (left >= kSlice) {
+#pragma unroll
+                            for (int k = 0; k < kSlice / 32; ++k) mma(s, k, id);
+                        } else {
+                            for (int k = 0; 32 * k < left; ++k) mma(s, k, id);
+                        }
                     }
                     tc_commit(&sm.empty[ring.i]);
                     if (last) tc_commit(&sm.sfempty[sf.i]);
-                    if (kt + 1 == p.nk) tc_commit(&sm.accfull[h]);
+                    if (end) tc_commit(&sm.accfull[h]);
                 }
                 __syncwarp();
                 ring.next();
@@ -510,6 +548,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = mbar_wait(&sm.itemempty[s], (uint32_t)((i / kItems) - 1) & 1u, &sm.abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
+            if constexpr (F8) {  // the rows' scale words, into L2 before warp 2 reads them
+                const uint8_t* b = p.xs + (int64_t)item.x0 * p.lxs;
+                for (int64_t o = 128 * lane; o < item.nx * p.lxs; o += 128 * 32)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
+            }
             if constexpr (GROUP) {
                 for (int c = lane; c < columns(item); c += 32) {
                     if (c >= item.nq) {
@@ -534,18 +577,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             ++i;
         };
-        auto queue_group = [&](const GroupAt& at, int64_t first, int64_t from, int64_t to) {
-            // tiles from .. to - 1 of the launch, of the group whose first one is `first`
-            int per, nqt;
-            group_tiles<NT>(at.len, at.m, &per, &nqt);
-            for (int64_t t = from; ok && t < to; t += GROUP ? 1 : gridDim.x) {
-                const int64_t xt = (t - first) / nqt, qt = (t - first) % nqt;
+        // tiles from, from + step, .. of a group
+        auto queue_group = [&](const GroupAt& at, const Tiles<NT>& g, int64_t from, int64_t to,
+                               unsigned step) {
+            for (int64_t t = from; ok && t < to; t += step) {
+                int64_t xt = t;
+                int32_t qt = 0;
+                if (g.nqt > 1) {
+                    xt = t / g.nqt;
+                    qt = (int32_t)(t - xt * g.nqt);
+                }
                 Item item;
                 item.j0 = xt * kM;
                 item.x0 = (int32_t)(at.l0 + item.j0);
                 item.nx = (int32_t)min((int64_t)kM, at.len - item.j0);
-                item.q0 = (int32_t)(at.p0 + qt * per);
-                item.nq = (int32_t)min((int64_t)per, at.m - qt * per);
+                item.q0 = (int32_t)(at.p0 + (int64_t)qt * g.per);
+                item.nq = (int32_t)min((int64_t)g.per, at.m - (int64_t)qt * g.per);
                 queue(item);
             }
         };
@@ -560,10 +607,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int64_t first = sm.prefix[lo];
                 for (int64_t g = lo * chunk; ok && g < p.g.ngroup && first < t1; g += 32) {
                     GroupAt at{0, 0, 0, 0};
-                    int per, nqt;
                     if (g + lane < p.g.ngroup) load_group(p, g + lane, &at);
-                    const int64_t tiles = group_tiles<NT>(at.len, at.m, &per, &nqt);
-                    int64_t incl = tiles;
+                    const int64_t weight = Tiles<NT>(at.len, at.m).weight();
+                    int64_t incl = weight;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -571,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const int64_t end = first + incl;
                     unsigned todo = __ballot_sync(0xffffffffu,
-                                                  tiles > 0 && end > t0 && end - tiles < t1);
+                                                  weight > 0 && end > t0 && end - weight < t1);
                     while (ok && todo) {
                         const int l = __ffs(todo) - 1;
                         todo &= todo - 1;
@@ -580,15 +626,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         o.len = __shfl_sync(0xffffffffu, at.len, l);
                         o.p0 = __shfl_sync(0xffffffffu, at.p0, l);
                         o.m = __shfl_sync(0xffffffffu, at.m, l);
-                        const int64_t e = __shfl_sync(0xffffffffu, end, l);
-                        const int64_t b = e - __shfl_sync(0xffffffffu, tiles, l);
-                        queue_group(o, b, max(b, t0), min(e, t1));
+                        const int64_t b = __shfl_sync(0xffffffffu, end - weight, l);
+                        const Tiles<NT> tiles(o.len, o.m);
+                        queue_group(o, tiles, tiles.first(t0 - b), tiles.first(t1 - b), 1);
                     }
                     first = __shfl_sync(0xffffffffu, end, 31);
                 }
             }
         } else {
-            queue_group(GroupAt{0, p.nx, 0, p.nq}, 0, blockIdx.x, total);
+            queue_group(GroupAt{0, p.nx, 0, p.nq}, Tiles<NT>(p.nx, p.nq), blockIdx.x, total,
+                        gridDim.x);
         }
         if (ok) queue(Item{0, 0, 0, 0, 0});
     } else if (warp < kQuery0) {
