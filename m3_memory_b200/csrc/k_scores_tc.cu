@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -42,20 +43,27 @@ constexpr int kEpi0 = 4;                // first epilogue warp (a multiple of 4)
 constexpr int kQuery0 = kEpi0 + kEpiWarps;
 constexpr int kItems = 8;               // tiles queued ahead
 
-// The two launch shapes: up to 64 queries a tile, for rows that are read for a few
-// queries each, with two slices a stage (a stage costs the MMA warp some 400 cycles
-// beside its MMAs), and up to 240 with one.
+// The launch shapes: up to NT queries a tile.  Rows and queries have rings of their
+// own (kX and kQ stages of kSlices slices; two slices a stage where the rows are read
+// for few queries, as a stage costs the MMA warp some 400 cycles beside its MMAs).
+// With up to 32 queries the queries' ring is the deeper one: gathered rows of q come
+// from anywhere in L2.
 template <int NT>
 struct Shape;
 template <>
+struct Shape<32> {
+    static constexpr int kX = 4, kQ = 8, kSlices = 2, kBox = 16, kAcc = 32, kTmem = 128,
+                         kSf0 = 64, kSfStep = 16;
+};
+template <>
 struct Shape<64> {
-    static constexpr int kStages = 4, kSlices = 2, kBox = 16, kAcc = 64, kTmem = 256, kSf0 = 128,
-                         kSfStep = 16;
+    static constexpr int kX = 4, kQ = 4, kSlices = 2, kBox = 16, kAcc = 64, kTmem = 256,
+                         kSf0 = 128, kSfStep = 16;
 };
 template <>
 struct Shape<240> {  // each accumulator's scales in the 16 columns behind it
-    static constexpr int kStages = 4, kSlices = 1, kBox = 48, kAcc = 256, kTmem = 512, kSf0 = 240,
-                         kSfStep = 256;
+    static constexpr int kX = 4, kQ = 4, kSlices = 1, kBox = 48, kAcc = 256, kTmem = 512,
+                         kSf0 = 240, kSfStep = 256;
 };
 
 struct Item {
@@ -69,13 +77,15 @@ constexpr int kSfSlots = 4;           // chunks of them in shared memory (two in
 
 template <int NT>
 struct alignas(1024) Smem {
-    unsigned char stage[Shape<NT>::kStages][Shape<NT>::kSlices][kXBytes + NT * kSlice];
+    unsigned char x[Shape<NT>::kX][Shape<NT>::kSlices][kXBytes];
+    unsigned char q[Shape<NT>::kQ][Shape<NT>::kSlices][NT * kSlice];
     unsigned char sf[kSfSlots][kSfBytes];
     int64_t at[kItems][NT];  // where each column's scores start; -1: nowhere
     alignas(16) int32_t row[kItems][NT];  // each column's row of q (0 where there is none)
     int64_t prefix[kThreads + 1];
     Item items[kItems];
-    uint64_t full[Shape<NT>::kStages], empty[Shape<NT>::kStages];
+    uint64_t xfull[Shape<NT>::kX], xempty[Shape<NT>::kX];
+    uint64_t qfull[Shape<NT>::kQ], qempty[Shape<NT>::kQ];
     uint64_t accfull[2], accempty[2], sffull[kSfSlots], sfempty[kSfSlots];
     uint64_t itemfull[kItems], itemempty[kItems], drain;
     int64_t warp_sum[kThreads / 32];
@@ -141,6 +151,7 @@ __device__ __forceinline__ uint32_t mx_idesc_byte(uint32_t idesc, int byte) {
 // A position in a ring of N slots and the parity of its current round.
 template <int N>
 struct Ring {
+    static constexpr uint32_t kSlots = N;
     uint32_t i = 0, phase = 0, n = 0;
     __device__ __forceinline__ void next() {
         ++n;
@@ -217,9 +228,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) tmem_alloc(&sm.tmem, S::kTmem);
     if (threadIdx.x == 32) {
-        for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(&sm.full[s], 2);  // the rows' and the queries' warps
-            mbar_init(&sm.empty[s], 1);
+        for (int s = 0; s < S::kX; ++s) {
+            mbar_init(&sm.xfull[s], 1);
+            mbar_init(&sm.xempty[s], 1);
+        }
+        for (int s = 0; s < S::kQ; ++s) {
+            mbar_init(&sm.qfull[s], 1);
+            mbar_init(&sm.qempty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&sm.accfull[s], 1);
@@ -310,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // tensor core by a fence that waits for all of the warp's, so each warp has
         // one stage in flight and the warps take the stages in turn.
         const unsigned char* src = static_cast<const unsigned char*>(p.q) + 16 * (lane & 7);
-        Ring<S::kStages> ring;
+        Ring<S::kQ> ring;
         bool ok = true;
         Item item;
         for (int64_t i = 0; ok && next_item(i, &item); ++i) {
@@ -318,16 +333,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int32_t* rows = sm.row[i % kItems];
             for (int kt = 0; kt < p.nk; kt += S::kSlices, ring.next()) {
                 if (ring.n % kQueryWarps != (uint32_t)(warp - kQuery0)) continue;
-                if (ring.n >= S::kStages &&
+                if (ring.n >= S::kQ &&
                     !__all_sync(0xffffffffu,
-                                mbar_wait(&sm.empty[ring.i], ring.phase ^ 1u, &sm.abort))) {
+                                mbar_wait(&sm.qempty[ring.i], ring.phase ^ 1u, &sm.abort))) {
                     ok = false;
                     break;
                 }
 #pragma unroll
                 for (int s = 0; s < S::kSlices; ++s) {
                     if (kt + s >= p.nk) break;
-                    const uint32_t dst = smem_u32(sm.stage[ring.i][s]) + kXBytes;
+                    const uint32_t dst = smem_u32(sm.q[ring.i][s]);
                     const int off = (kt + s) * kSlice;
                     const int left = p.row_bytes - off - 16 * (lane & 7);
                     const uint32_t size = left >= 16 ? 16u : left > 0 ? (uint32_t)left : 0u;
@@ -341,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 cp_async_wait_all();
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.full[ring.i]);
+                if (lane == 0) mbar_arrive(&sm.qfull[ring.i]);
             }
             done_with(i);
         }
@@ -350,61 +365,69 @@ __global__ void __launch_bounds__(kThreads, 1)
         // its issuer some 100 cycles).  The warp walks the tiles with warp-uniform
         // values, so the copies' operands stay in uniform registers; the elected lane
         // issues.
-        const bool leader = elect_one(), xside = warp == 0;
-        Ring<S::kStages> ring;
-        bool ok = true;
-        Item item;
-        for (int64_t i = 0; ok && next_item(i, &item); ++i) {
-            const int qboxes = (columns(item) + S::kBox - 1) / S::kBox;
-            const int xboxes = item.nx > 96 ? 0 : (item.nx + 31) / 32;
-            const uint32_t bytes =
-                (uint32_t)kSlice * (xside ? (xboxes ? xboxes * 32 : kM) : qboxes * S::kBox);
-            done_with(i);
-            for (int kt = 0; kt < p.nk; kt += S::kSlices) {
-                if (ring.n >= S::kStages &&
-                    !__all_sync(0xffffffffu,
-                                mbar_wait(&sm.empty[ring.i], ring.phase ^ 1u, &sm.abort))) {
-                    ok = false;
-                    break;
-                }
-                if (leader) {
-                    uint64_t* bar = &sm.full[ring.i];
-                    const int ns = min(S::kSlices, p.nk - kt);
-                    mbar_arrive_expect_tx(bar, bytes * ns);
-                    for (int s = 0; s < ns; ++s) {
-                        unsigned char* sx = sm.stage[ring.i][s];
-                        unsigned char* sq = sx + kXBytes;
-                        const int x = (kt + s) * (F8 ? kSlice : kSlice / 2);
-                        if (!xside) {
-                            for (int b = 0; b < qboxes; ++b)
-                                tma_load_2d(sq + b * S::kBox * kSlice, &map_q, x,
-                                            item.q0 + b * S::kBox, bar);
-                        } else if (xboxes == 0) {
-                            tma_load_2d(sx, &map_x, x, item.x0, bar);
-                        } else {
-                            for (int b = 0; b < xboxes; ++b)
-                                tma_load_2d(sx + b * 32 * kSlice, &map_x32, x, item.x0 + 32 * b,
-                                            bar);
-                        }
+        const bool leader = elect_one();
+        auto load = [&](auto ring, uint64_t* full, uint64_t* empty, auto boxes_of, auto copy) {
+            constexpr uint32_t N = decltype(ring)::kSlots;
+            bool ok = true;
+            Item item;
+            for (int64_t i = 0; ok && next_item(i, &item); ++i) {
+                done_with(i);
+                const uint32_t bytes = (uint32_t)kSlice * boxes_of(item);
+                for (int kt = 0; kt < p.nk; kt += S::kSlices) {
+                    if (ring.n >= N &&
+                        !__all_sync(0xffffffffu,
+                                    mbar_wait(&empty[ring.i], ring.phase ^ 1u, &sm.abort))) {
+                        ok = false;
+                        break;
                     }
+                    if (leader) {
+                        const int ns = min(S::kSlices, p.nk - kt);
+                        mbar_arrive_expect_tx(&full[ring.i], bytes * ns);
+                        for (int s = 0; s < ns; ++s)
+                            copy(item, ring.i, s, (kt + s) * (F8 ? kSlice : kSlice / 2));
+                    }
+                    __syncwarp();
+                    ring.next();
                 }
-                __syncwarp();
-                ring.next();
             }
+            // no copy may still be landing when the CTA leaves
+            if (leader)
+                for (uint32_t k = ring.n > N ? ring.n - N : 0u; k < ring.n; ++k)
+                    mbar_drain(&full[k % N], (k / N) & 1u);
+            __syncwarp();
+        };
+        if (warp == 0) {
+            // the 32-row boxes of a tile of less than four (0: one box of 128 rows)
+            auto small = [](const Item& it) { return it.nx > 96 ? 0 : (it.nx + 31) / 32; };
+            load(
+                Ring<S::kX>(), sm.xfull, sm.xempty,
+                [&](const Item& it) { return small(it) ? 32 * small(it) : kM; },
+                [&](const Item& it, uint32_t slot, int s, int x) {
+                    const int n = small(it);
+                    if (n == 0) tma_load_2d(sm.x[slot][s], &map_x, x, it.x0, &sm.xfull[slot]);
+                    for (int b = 0; b < n; ++b)
+                        tma_load_2d(sm.x[slot][s] + b * 32 * kSlice, &map_x32, x, it.x0 + 32 * b,
+                                    &sm.xfull[slot]);
+                });
+        } else {
+            auto boxes = [&](const Item& it) { return (columns(it) + S::kBox - 1) / S::kBox; };
+            load(
+                Ring<S::kQ>(), sm.qfull, sm.qempty,
+                [&](const Item& it) { return boxes(it) * S::kBox; },
+                [&](const Item& it, uint32_t slot, int s, int x) {
+                    for (int b = 0; b < boxes(it); ++b)
+                        tma_load_2d(sm.q[slot][s] + b * S::kBox * kSlice, &map_q, x,
+                                    it.q0 + b * S::kBox, &sm.qfull[slot]);
+                });
         }
-        // no copy may still be landing when the CTA leaves (where the other warp gave
-        // up first, the stage never fills and the wait ends at its limit)
-        if (leader)
-            for (uint32_t k = ring.n > S::kStages ? ring.n - S::kStages : 0u; k < ring.n; ++k)
-                mbar_drain(&sm.full[k % S::kStages], (k / S::kStages) & 1u);
-        __syncwarp();
     } else if (warp == 1) {
         // ---- MMAs: tile i accumulates in TMEM half i & 1.  Warp-uniform like the loads.
         const bool leader = elect_one();
-        // descriptors of the first stage; an offset of b bytes adds b >> 4
-        const uint64_t dx0 = sw128_desc(smem_u32(sm.stage[0][0]));
-        constexpr uint32_t kStep = (kXBytes + NT * kSlice) >> 4;  // a slice
-        Ring<S::kStages> ring;
+        // descriptors of the first stages; an offset of b bytes adds b >> 4
+        const uint64_t dx0 = sw128_desc(smem_u32(sm.x[0][0]));
+        const uint64_t dq0 = sw128_desc(smem_u32(sm.q[0][0]));
+        Ring<S::kX> rx;
+        Ring<S::kQ> rq;
         Ring<kSfSlots> sf;
         bool ok = true;
         Item item;
@@ -431,7 +454,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         go = mbar_wait(&sm.sfempty[(sf.n - 2) % kSfSlots],
                                        ((sf.n - 2) / kSfSlots) & 1u, &sm.abort);
                 }
-                go = go && mbar_wait(&sm.full[ring.i], ring.phase, &sm.abort);
+                go = go && mbar_wait(&sm.qfull[rq.i], rq.phase, &sm.abort);
+                go = go && mbar_wait(&sm.xfull[rx.i], rx.phase, &sm.abort);
                 if (!__all_sync(0xffffffffu, go)) {
                     ok = false;
                     break;
@@ -445,8 +469,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (NT > 128) tc_copy_scales(tsf + 8, src + 1024);
                     }
                     auto mma = [&](int s, int k, uint32_t id) {
-                        const uint64_t a = dx0 + (ring.i * S::kSlices + s) * kStep + 2 * k;
-                        const uint64_t b = a + (kXBytes >> 4);
+                        const uint64_t a =
+                            dx0 + (rx.i * S::kSlices + s) * (kXBytes >> 4) + 2 * k;
+                        const uint64_t b =
+                            dq0 + (rq.i * S::kSlices + s) * (NT * kSlice >> 4) + 2 * k;
                         if (F8) tc_mma_mx(d, a, b, id, tsf, tsf + 4, (kt | s | k) != 0);
                         else tc_mma_f16(d, a, b, id, (kt | s | k) != 0);
                     };
@@ -461,12 +487,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int k = 0; 32 * k < left; ++k) mma(s, k, id);
                         }
                     }
-                    tc_commit(&sm.empty[ring.i]);
+                    tc_commit(&sm.xempty[rx.i]);
+                    tc_commit(&sm.qempty[rq.i]);
                     if (last) tc_commit(&sm.sfempty[sf.i]);
                     if (end) tc_commit(&sm.accfull[h]);
                 }
                 __syncwarp();
-                ring.next();
+                rx.next();
+                rq.next();
                 if (last) sf.next();
             }
         }
@@ -721,21 +749,20 @@ cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* 
 }
 
 template <bool GROUP>
-cudaError_t launch_any(const m3g_rows& q, const m3g_rows& x, const Params& p, bool wide, void* out,
-                       int out_dtype, unsigned grid, cudaStream_t st) {
+cudaError_t launch_any(const m3g_rows& q, const m3g_rows& x, const Params& p, int64_t queries,
+                       void* out, int out_dtype, unsigned grid, cudaStream_t st) {
     const bool f32 = out_dtype == M3G_F32;
-    if (x.dtype == M3G_E4M3) {
-        if (wide)
-            return f32 ? launch<true, 240, GROUP, float>(q, x, p, out, grid, st)
-                       : launch<true, 240, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
-        return f32 ? launch<true, 64, GROUP, float>(q, x, p, out, grid, st)
-                   : launch<true, 64, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
-    }
-    if (wide)
-        return f32 ? launch<false, 240, GROUP, float>(q, x, p, out, grid, st)
-                   : launch<false, 240, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
-    return f32 ? launch<false, 64, GROUP, float>(q, x, p, out, grid, st)
-               : launch<false, 64, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+    auto with = [&](auto nt) {
+        constexpr int NT = decltype(nt)::value;
+        if (x.dtype == M3G_E4M3)
+            return f32 ? launch<true, NT, GROUP, float>(q, x, p, out, grid, st)
+                       : launch<true, NT, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+        return f32 ? launch<false, NT, GROUP, float>(q, x, p, out, grid, st)
+                   : launch<false, NT, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+    };
+    if (queries <= 32) return with(std::integral_constant<int, 32>());
+    if (queries <= 64) return with(std::integral_constant<int, 64>());
+    return with(std::integral_constant<int, 240>());
 }
 
 Params params_of(const m3g_rows& q, const m3g_rows& x, float alpha, float beta, int* err) {
@@ -763,9 +790,8 @@ cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha,
                               cudaStream_t st) {
     Params p = params_of(q, x, alpha, beta, err);
     p.ld_out = ld_out;
-    const bool wide = q.n > 64;
     const int64_t tiles = (x.n + kM - 1) / kM * ((q.n + 15) / 16);  // at least as many as there are
-    return launch_any<false>(q, x, p, wide, out, out_dtype,
+    return launch_any<false>(q, x, p, q.n, out, out_dtype,
                              (unsigned)std::min<int64_t>(tiles, sms), st);
 }
 
@@ -774,8 +800,7 @@ cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const Score
                                int sms, cudaStream_t st) {
     Params p = params_of(q, x, alpha, beta, err);
     p.g = g;
-    const bool wide = g.npair / g.ngroup > 64;
-    return launch_any<true>(q, x, p, wide, out, out_dtype, (unsigned)sms, st);
+    return launch_any<true>(q, x, p, g.npair / g.ngroup, out, out_dtype, (unsigned)sms, st);
 }
 
 }  // namespace m3g
