@@ -17,8 +17,8 @@
 //
 // A launch is one CTA per SM.  A tile is 128 rows of a group and up to NT of its
 // queries, queries fastest, so the rows come from L2 after their first tile.  Warp 0 loads rows and warp 12 queries (TMA; those of a group
-// are gathered by warps 12-15), warp 1 issues the MMAs, warp 2 brings scale words, warp 3 walks the
-// groups and queues tiles, warps 4-11 store.  Every wait is bounded.
+// are gathered by warps 12-15), warp 1 issues the MMAs, warp 3 walks the groups and
+// queues tiles, warps 4-11 store, warps 16-19 bring scale words.  Every wait is bounded.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -38,9 +38,11 @@ constexpr int kSlice = 128;             // bytes of a row a swizzled tile holds 
 constexpr int kXBytes = kM * kSlice;
 constexpr int kEpiWarps = 8;            // two for each quarter of the TMEM lanes
 constexpr int kQueryWarps = 4;          // each gathers every fourth stage's queries
-constexpr int kThreads = (4 + kEpiWarps + kQueryWarps) * 32;
+constexpr int kScaleWarps = 4;          // one for each quarter of the TMEM lanes
+constexpr int kThreads = (4 + kEpiWarps + kQueryWarps + kScaleWarps) * 32;
 constexpr int kEpi0 = 4;                // first epilogue warp (a multiple of 4)
 constexpr int kQuery0 = kEpi0 + kEpiWarps;
+constexpr int kScale0 = kQuery0 + kQueryWarps;  // (a multiple of 4)
 constexpr int kItems = 8;               // tiles queued ahead
 
 // The launch shapes: up to NT queries a tile.  Rows and queries have rings of their
@@ -53,17 +55,17 @@ struct Shape;
 template <>
 struct Shape<32> {
     static constexpr int kX = 4, kQ = 8, kSlices = 2, kBox = 16, kAcc = 32, kTmem = 128,
-                         kSf0 = 64, kSfStep = 16;
+                         kSf = 4, kSf0 = 64, kSfStep = 8;
 };
 template <>
 struct Shape<64> {
     static constexpr int kX = 4, kQ = 4, kSlices = 2, kBox = 16, kAcc = 64, kTmem = 256,
-                         kSf0 = 128, kSfStep = 16;
+                         kSf = 4, kSf0 = 128, kSfStep = 8;
 };
 template <>
 struct Shape<240> {  // each accumulator's scales in the 16 columns behind it
     static constexpr int kX = 4, kQ = 4, kSlices = 1, kBox = 48, kAcc = 256, kTmem = 512,
-                         kSf0 = 240, kSfStep = 256;
+                         kSf = 2, kSf0 = 240, kSfStep = 256;
 };
 
 struct Item {
@@ -72,21 +74,17 @@ struct Item {
     int64_t j0;      // the first row's place in its list
 };
 
-constexpr int kSfBytes = 512 + 1024;  // scale words of a 512-dim chunk: x rows, queries
-constexpr int kSfSlots = 4;           // chunks of them in shared memory (two in TMEM)
-
 template <int NT>
 struct alignas(1024) Smem {
     unsigned char x[Shape<NT>::kX][Shape<NT>::kSlices][kXBytes];
     unsigned char q[Shape<NT>::kQ][Shape<NT>::kSlices][NT * kSlice];
-    unsigned char sf[kSfSlots][kSfBytes];
     int64_t at[kItems][NT];  // where each column's scores start; -1: nowhere
     alignas(16) int32_t row[kItems][NT];  // each column's row of q (0 where there is none)
     int64_t prefix[kThreads + 1];
     Item items[kItems];
     uint64_t xfull[Shape<NT>::kX], xempty[Shape<NT>::kX];
     uint64_t qfull[Shape<NT>::kQ], qempty[Shape<NT>::kQ];
-    uint64_t accfull[2], accempty[2], sffull[kSfSlots], sfempty[kSfSlots];
+    uint64_t accfull[2], accempty[2], sffull[Shape<NT>::kSf], sfempty[Shape<NT>::kSf];
     uint64_t itemfull[kItems], itemempty[kItems], drain;
     int64_t warp_sum[kThreads / 32];
     uint32_t tmem;
@@ -127,15 +125,15 @@ __device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, ui
         : "memory");
 }
 
-// 32 rows of 16 bytes from shared memory to four TMEM columns, repeated in each of
-// the four lane quarters: the words of rows r, r + 32, r + 64, r + 96 are row r's 16
-// bytes.  No swizzle; 8 rows of 16 bytes every 128 bytes.
-__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint32_t saddr) {
-    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(128 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d)
+// One word a lane into each of four TMEM columns of the warp's lane quarter.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c,
+                                         uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
+                 "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // kind::mxf8f6f4: both operands e4m3 (0) and K-major, N >> 3 at bits 17-22, ue8m0
@@ -151,7 +149,7 @@ __device__ __forceinline__ uint32_t mx_idesc_byte(uint32_t idesc, int byte) {
 // A position in a ring of N slots and the parity of its current round.
 template <int N>
 struct Ring {
-    static constexpr uint32_t kSlots = N;
+    __device__ static constexpr uint32_t slots() { return N; }
     uint32_t i = 0, phase = 0, n = 0;
     __device__ __forceinline__ void next() {
         ++n;
@@ -240,14 +238,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sm.accfull[s], 1);
             mbar_init(&sm.accempty[s], kEpiWarps);
         }
-        for (int s = 0; s < kSfSlots; ++s) {
-            mbar_init(&sm.sffull[s], 1);
+        for (int s = 0; s < S::kSf; ++s) {
+            mbar_init(&sm.sffull[s], kScaleWarps);
             mbar_init(&sm.sfempty[s], 1);
         }
         for (int s = 0; s < kItems; ++s) {
             mbar_init(&sm.itemfull[s], 1);
             // its readers' warps: rows, MMAs, scales, epilogue, queries
-            mbar_init(&sm.itemempty[s], 2 + (F8 ? 1 : 0) + kEpiWarps +
+            mbar_init(&sm.itemempty[s], 2 + (F8 ? kScaleWarps : 0) + kEpiWarps +
                                             (GROUP && p.g.pair_row ? kQueryWarps : 1));
         }
         mbar_init(&sm.drain, 1);
@@ -318,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool gather = GROUP && p.g.pair_row != nullptr;
     auto columns = [](const Item& it) { return (it.nq + 15) & ~15; };
 
-    if (warp >= kQuery0 && gather) {
+    if (warp >= kQuery0 && warp < kScale0 && gather) {
         // ---- a group's queries, gathered with 16-byte copies (TMA's gather4 takes
         // some 230 cycles for its four rows): eight lanes a row, four rows a copy, in
         // the 128-byte swizzle the MMA reads.  The copies are made visible to the
@@ -367,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // issues.
         const bool leader = elect_one();
         auto load = [&](auto ring, uint64_t* full, uint64_t* empty, auto boxes_of, auto copy) {
-            constexpr uint32_t N = decltype(ring)::kSlots;
+            constexpr uint32_t N = decltype(ring)::slots();
             bool ok = true;
             Item item;
             for (int64_t i = 0; ok && next_item(i, &item); ++i) {
@@ -428,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t dq0 = sw128_desc(smem_u32(sm.q[0][0]));
         Ring<S::kX> rx;
         Ring<S::kQ> rq;
-        Ring<kSfSlots> sf;
+        Ring<S::kSf> sf;
         bool ok = true;
         Item item;
         for (int64_t i = 0; ok && next_item(i, &item); ++i) {
@@ -445,15 +443,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool first = F8 && (kt & 3) == 0;
                 const bool end = kt + S::kSlices >= p.nk;
                 const bool last = F8 && (((kt + S::kSlices) & 3) == 0 || end);
-                const uint32_t tsf = tmem + (uint32_t)(S::kSf0 + (int)(sf.n & 1u) * S::kSfStep);
+                const uint32_t tsf = tmem + (uint32_t)(S::kSf0 + (int)sf.i * S::kSfStep);
                 bool go = true;
-                if (first) {
-                    // the chunk's words, and its place in TMEM (the chunk two before it)
-                    go = mbar_wait(&sm.sffull[sf.i], sf.phase, &sm.abort);
-                    if (go && sf.n >= 2)
-                        go = mbar_wait(&sm.sfempty[(sf.n - 2) % kSfSlots],
-                                       ((sf.n - 2) / kSfSlots) & 1u, &sm.abort);
-                }
+                if (first) go = mbar_wait(&sm.sffull[sf.i], sf.phase, &sm.abort);
                 go = go && mbar_wait(&sm.qfull[rq.i], rq.phase, &sm.abort);
                 go = go && mbar_wait(&sm.xfull[rx.i], rx.phase, &sm.abort);
                 if (!__all_sync(0xffffffffu, go)) {
@@ -462,12 +454,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after();
                 if (leader) {
-                    if (first) {
-                        const uint32_t src = smem_u32(sm.sf[sf.i]);
-                        tc_copy_scales(tsf, src);
-                        tc_copy_scales(tsf + 4, src + 512);
-                        if (NT > 128) tc_copy_scales(tsf + 8, src + 1024);
-                    }
                     auto mma = [&](int s, int k, uint32_t id) {
                         const uint64_t a =
                             dx0 + (rx.i * S::kSlices + s) * (kXBytes >> 4) + 2 * k;
@@ -504,15 +490,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_drain(&sm.drain, 0);
         }
         __syncwarp();
-    } else if (warp == 2) {
+    } else if (warp >= kScale0) {
         if constexpr (F8) {
-            // ---- scale words, read one chunk ahead of the one being handed over:
-            // lane r brings rows r, r + 32, ..
+            // ---- scale words, read one chunk ahead of the one being handed over, from
+            // global memory to TMEM: the four columns of 128 rows hold rows r, r + 32,
+            // r + 64, r + 96 in lane r, the same in each lane quarter, so each of these
+            // warps stores the same words to its own.
             constexpr int W = 4 + (NT > 128 ? 8 : 4);
             const uint8_t* ptr[W];
             uint32_t next[W];
+            const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            Ring<S::kSf> sf;
             Item item;
-            int64_t i = 0, sf = 0;
+            int64_t i = 0;
             auto load = [&](int kt) {
 #pragma unroll
                 for (int u = 0; u < W; ++u)
@@ -538,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return true;
             };
             bool ok = open();
-            for (int kt = 0; ok; ++sf) {
+            for (int kt = 0; ok; sf.next()) {
                 uint32_t w[W];
 #pragma unroll
                 for (int u = 0; u < W; ++u) w[u] = next[u];
@@ -550,19 +540,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     kt = 0;
                     more = open();
                 }
-                const int c = (int)(sf % kSfSlots);
-                if (sf >= kSfSlots)
-                    ok = mbar_wait(&sm.sfempty[c], (uint32_t)((sf / kSfSlots) - 1) & 1u,
-                                   &sm.abort);
+                if (sf.n >= S::kSf)
+                    ok = mbar_wait(&sm.sfempty[sf.i], sf.phase ^ 1u, &sm.abort);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = quarter + (uint32_t)(S::kSf0 + (int)sf.i * S::kSfStep);
 #pragma unroll
                 for (int u = 0; u < W; u += 4)
-                    *reinterpret_cast<uint4*>(sm.sf[c] + 128 * u + 16 * lane) =
-                        make_uint4(w[u], w[u + 1], w[u + 2], w[u + 3]);
-                fence_proxy_async_smem();
+                    tmem_st4(at + u, w[u], w[u + 1], w[u + 2], w[u + 3]);
+                tmem_st_wait();
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.sffull[c]);
+                if (lane == 0) mbar_arrive(&sm.sffull[sf.i]);
                 ok = more;
             }
         }
@@ -576,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = mbar_wait(&sm.itemempty[s], (uint32_t)((i / kItems) - 1) & 1u, &sm.abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
-            if constexpr (F8) {  // the rows' scale words, into L2 before warp 2 reads them
+            if constexpr (F8) {  // the rows' scale words, into L2 before they are read
                 const uint8_t* b = p.xs + (int64_t)item.x0 * p.lxs;
                 for (int64_t o = 128 * lane; o < item.nx * p.lxs; o += 128 * 32)
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
@@ -666,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         gridDim.x);
         }
         if (ok) queue(Item{0, 0, 0, 0, 0});
-    } else if (warp < kQuery0) {
+    } else if (warp >= kEpi0 && warp < kQuery0) {
         // ---- epilogue: warp w holds TMEM lanes 32 (w & 3) .. of the tile's rows, and
         // every other 16 columns
         const int quarter = warp & 3, half = (warp - kEpi0) >> 2;
