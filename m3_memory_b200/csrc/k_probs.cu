@@ -1,9 +1,28 @@
-// k_probs.cu -- scores as probabilities: log-sum-exp, entropy, the log
-// probability of given entries and the k most probable ones.
+// k_probs.cu -- scores as probabilities: log-sum-exp, entropy, the log probability
+// of given entries and the k most probable ones, in one pass over the scores.
+//
+// With t = score (scale > 0) or -score, c = |scale| and l = c t, a part of a row is
+// summed up as (m, z, w): its largest t, z = sum e^d and w = sum d e^d, where
+// d = c t - c m.  Parts join by M = max m, z' = e^(c m - c M) z and
+// w' = e^(c m - c M) (w + (c m - c M) z); then logsumexp = c M + log z and
+// entropy = log z - w / z.  d is one fma on c m as rounded, so the formulas hold
+// exactly whatever that rounding was.  Entries that are NaN, or -inf after scaling,
+// come out of max(d, -1000) with e^d = 0.
+//
+// The best k of a row pass through a buffer in shared memory: a thread offers the
+// entries of its 16 that reach the current bound tau, a lower bound of the k-th
+// best.  tau first comes from the threads' own maxima (at least k of them reach the
+// smallest of the warps' ceil(k / 8)-th largest), later from the buffer itself, which
+// is cut to its best k when it could overflow.
+//
+// The scores' bytes bound it.  A block of 256 threads takes a row, or one of P parts
+// of it where rows are few; parts leave (m, z, w) and their best k in the caller's
+// scratch and a second kernel joins them.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "kernels_scores.h"
@@ -11,121 +30,430 @@
 namespace m3g {
 namespace {
 
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kPer = 16;                      // entries a thread holds of a tile
+constexpr int kTile = kThreads * kPer;
+constexpr int kBuf = kTile + kProbsMaxK;      // a tile always fits behind the best k
+constexpr unsigned long long kNone = ~0ull;   // no entry
+
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+
+struct Sums {
+    float m = -INFINITY, z = 0.f, w = 0.f;
+};
+
+__device__ __forceinline__ float exp_of(float d) { return exp2f(d * 1.4426950408889634f); }
+
+// a part's sums taken to another reference value
+__device__ __forceinline__ void rebase(Sums& s, float c, float m) {
+    if (s.m == m || s.z == 0.f) {
+        s.m = m;
+        return;
+    }
+    const float d = fmaxf(c * s.m - c * m, -1000.f), f = exp_of(d);
+    s.w = f * fmaf(d, s.z, s.w);
+    s.z *= f;
+    s.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    rebase(a, c, m);
+    rebase(b, c, m);
+    a.z += b.z;
+    a.w += b.w;
+    return a;
+}
+
+struct Shared {
+    unsigned long long buf[kBuf], best[kProbsMaxK];
+    Sums sums[kWarps];
+    float offer[kWarps];
+    int count;
+};
+
+// One value for each warp, the sums of all its lanes in fixed order.
+__device__ __forceinline__ Sums warp_join(Sums s, float c) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Sums b;
+        b.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+        b.z = __shfl_xor_sync(0xffffffffu, s.z, o);
+        b.w = __shfl_xor_sync(0xffffffffu, s.w, o);
+        s = join(s, b, c);
+    }
+    return s;
+}
+
+__device__ __forceinline__ Sums block_join(Sums s, float c, Shared& sm) {
+    s = warp_join(s, c);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm.sums[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = sm.sums[0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) s = join(s, sm.sums[i], c);
+    return s;
+}
+
+// Bitonic sort of one float a lane, descending.
+__device__ __forceinline__ float warp_sort_desc(float v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const float p = __shfl_xor_sync(0xffffffffu, v, j);
+            v = (((lane & k) == 0) == ((lane & j) == 0)) ? fmaxf(v, p) : fminf(v, p);
+        }
+    return v;
+}
+
+// A value that at least k of the threads' v reach (all of them if fewer than k are
+// above -inf): the smallest of the warps' ceil(k / kWarps)-th largest.
+__device__ __forceinline__ float offered_bound(float v, int k, Shared& sm) {
+    v = warp_sort_desc(v);
+    const int nth = (k + kWarps - 1) / kWarps - 1;
+    if ((threadIdx.x & 31) == nth) sm.offer[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float b = sm.offer[0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) b = fminf(b, sm.offer[i]);
+    __syncthreads();
+    return b;
+}
+
+// Keys order entries best first: descending t, then ascending place.
+__device__ __forceinline__ unsigned long long key_of(float t, uint32_t place) {
+    return ((unsigned long long)float_key(-t) << 32) | place;
+}
+__device__ __forceinline__ float t_of(unsigned long long key) {
+    return -key_float((uint32_t)(key >> 32));
+}
+
+// Appends the keys a thread passes (any of them kNone) to the buffer.
+__device__ __forceinline__ void append(unsigned long long key, Shared& sm) {
+    if (key != kNone) sm.buf[atomicAdd(&sm.count, 1)] = key;
+}
+
+// Cuts the buffer's n entries to their best min(k, n), sorted, and returns the
+// number.  Every entry's place is the number of better ones, counted among the
+// entries that reach a bound of the k-th best: first the warps' offers of the
+// threads' best ones, then, where many entries still reach that (rows in ascending
+// order), the exact k-th of them.
+__device__ __noinline__ int best_of_buffer(int n, int k, Shared& sm) {
+    const int tid = threadIdx.x;
+    for (int pass = 0; pass < 2 && n > kThreads && n > 4 * k; ++pass) {
+        unsigned long long mine[kBuf / kThreads + 1], best = kNone;
+#pragma unroll
+        for (int u = 0; u < kBuf / kThreads + 1; ++u) {
+            const int i = tid + u * kThreads;
+            mine[u] = i < n ? sm.buf[i] : kNone;
+            best = min(best, mine[u]);
+        }
+        unsigned long long bound = kNone;  // entries above it are dropped
+        if (pass == 0) {
+            const float b = offered_bound(best == kNone ? ninf() : t_of(best), k, sm);
+            if (b > ninf()) bound = key_of(b, 0xFFFFFFFFu);
+        } else {
+            __syncthreads();
+            sm.buf[tid] = best;
+            __syncthreads();
+            int better = 0;
+            for (int i = 0; i < kThreads; ++i) better += sm.buf[i] < best;
+            // (n > kThreads, so every thread has a best one and they are distinct)
+            if (better == k - 1) sm.buf[kThreads] = best;
+            __syncthreads();
+            bound = sm.buf[kThreads];
+        }
+        __syncthreads();
+        if (tid == 0) sm.count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kBuf / kThreads + 1; ++u)
+            append(mine[u] <= bound ? mine[u] : kNone, sm);
+        __syncthreads();
+        n = sm.count;
+        __syncthreads();
+    }
+    // places among the n entries that are left
+    const int kept = min(n, k);
+    for (int i0 = tid; i0 < n; i0 += kThreads) {
+        const unsigned long long key = sm.buf[i0];
+        int better = 0;
+        for (int i = 0; i < n; ++i) better += sm.buf[i] < key;
+        if (better < k) sm.best[better] = key;
+    }
+    __syncthreads();
+    if (tid < kept) sm.buf[tid] = sm.best[tid];
+    if (tid == 0) sm.count = kept;
+    __syncthreads();
+    return kept;
+}
+
+// ---------------- a part of a row ----------------
+
+template <class T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int kN = 4;
+    __device__ static void unpack(const uint4& r, float* o) {
+        o[0] = __uint_as_float(r.x);
+        o[1] = __uint_as_float(r.y);
+        o[2] = __uint_as_float(r.z);
+        o[3] = __uint_as_float(r.w);
+    }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    __device__ static void unpack(const uint4& r, float* o) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = __uint_as_float(w[i] << 16);
+            o[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+
 __device__ __forceinline__ float load_score(const float* p) { return *p; }
 __device__ __forceinline__ float load_score(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// Scores oriented so that larger is more probable: t = score for scale > 0, -score
-// else, with c = |scale|; l = c t.  An entry takes part if l is not NaN or -inf.
-__device__ __forceinline__ bool takes_part(float t, float c) {
-    return c * t > __int_as_float(0xff800000);
+// The 16 bytes of granule g of a row whose first entry is `mis` entries into its
+// first granule; entries outside the row are NaN.
+template <class T>
+__device__ __forceinline__ uint4 load_granule(const T* row, int64_t len, int mis, int64_t g) {
+    constexpr int V = Vec<T>::kN;
+    const int64_t i = g * V - mis;
+    if (i >= 0 && i + V <= len) return __ldcs(reinterpret_cast<const uint4*>(row + i));
+    uint4 r = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaNs of either type
+    if (i + V > 0 && i < len) {
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+            if (i + u >= 0 && i + u < len) e[u] = row[i + u];
+    }
+    return r;
 }
 
-// One block per row; 256 threads.
+struct RowAt {
+    int64_t first, len;
+};
+__device__ __forceinline__ RowAt row_at(const ProbsArgs& a, int64_t row) {
+    if (!a.row_off) return {row * a.ld, a.n};
+    const int64_t b = max((int64_t)0, min(a.row_off[row], a.n));
+    const int64_t len = max((int64_t)0, min(a.row_off[row + 1], a.n) - b);
+    return {b, min(len, (int64_t)INT32_MAX)};
+}
+
+// l = c t, or the reference value where that is infinite
+__device__ __forceinline__ float log_prob(float t, float c, float cm, float logz) {
+    const float l = c * t;
+    if (!(l > ninf())) return ninf();  // left out
+    if (cm == __int_as_float(0x7f800000)) return l == cm ? __int_as_float(0x7fc00000) : ninf();
+    return fmaf(c, t, -cm) - logz;
+}
+
+// The answer of a row from its sums and its best entries (in sm.buf, sorted).
 template <class T>
-__global__ void __launch_bounds__(256) score_probs_kernel(ProbsArgs a) {
-    __shared__ float red[256], red2[256];
-    __shared__ unsigned long long redk[256];
+__device__ void finish_row(const ProbsArgs& a, int64_t row, const RowAt& at, const Sums& s,
+                           int kept, float c, float sgn, Shared& sm) {
+    const float cm = s.z > 0.f || s.m > ninf() ? c * s.m : ninf();
+    const bool inf = cm == __int_as_float(0x7f800000);
+    const float logz = logf(s.z);
+    if (threadIdx.x == 0) {
+        a.lse[row] = inf || !(s.z > 0.f) ? cm : cm + logz;
+        a.entropy[row] = inf          ? __int_as_float(0x7fc00000)
+                         : s.z > 0.f ? fmaxf(logz - s.w / s.z, 0.f)  // (roundings aside)
+                                     : 0.f;
+    }
+    const T* x = static_cast<const T*>(a.scores) + at.first;
+    for (int j = threadIdx.x; j < a.ngiven; j += kThreads) {
+        const int64_t g = a.given[row * a.ngiven + j];
+        a.out_given[row * a.ngiven + j] =
+            g >= 0 && g < at.len ? log_prob(sgn * load_score(x + g), c, cm, logz) : ninf();
+    }
+    for (int j = threadIdx.x; j < a.k; j += kThreads) {
+        const unsigned long long key = j < kept ? sm.buf[j] : kNone;
+        a.top_index[row * a.k + j] = key == kNone ? -1 : (int64_t)(uint32_t)key;
+        a.top[row * a.k + j] = key == kNone ? ninf() : log_prob(t_of(key), c, cm, logz);
+    }
+    __syncthreads();
+}
+
+// A part's place in the scratch: its sums, then its best k keys.
+__device__ __forceinline__ unsigned char* part_at(const ProbsArgs& a, int64_t unit) {
+    return static_cast<unsigned char*>(a.work) + unit * (16 + 8 * (int64_t)a.k);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads, 4) score_probs_kernel(ProbsArgs a, int parts) {
+    constexpr int V = Vec<T>::kN, kVecs = kPer / V;
+    __shared__ Shared sm;
     const int tid = threadIdx.x;
     const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
-    for (int64_t row = blockIdx.x; row < a.nq; row += gridDim.x) {
-        int64_t b = row * a.ld, len = a.n;
-        if (a.row_off) {
-            b = max((int64_t)0, min(a.row_off[row], a.n));
-            len = max((int64_t)0, min(a.row_off[row + 1], a.n) - b);
+    for (int64_t unit = blockIdx.x; unit < a.nq * parts; unit += gridDim.x) {
+        const int64_t row = unit / parts;
+        const int part = (int)(unit - row * parts);
+        const RowAt at = row_at(a, row);
+        const T* x = static_cast<const T*>(a.scores) + at.first;
+        const int mis = (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % V);
+        const int64_t ngran = (at.len + mis + V - 1) / V;
+        const int64_t g0 = ngran * part / parts, g1 = ngran * (part + 1) / parts;
+        Sums s;
+        float tau = ninf();  // entries below it are not among the best k
+        if (tid == 0) sm.count = 0;
+        uint4 raw[kVecs];
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+            const int64_t g = g0 + v * kThreads + tid;
+            raw[v] = g < g1 ? load_granule(x, at.len, mis, g) : make_uint4(~0u, ~0u, ~0u, ~0u);
         }
-        const T* s = static_cast<const T*>(a.scores) + b;
-        float m = __int_as_float(0xff800000);
-        for (int64_t i = tid; i < len; i += 256) {
-            const float t = sgn * load_score(s + i);
-            if (takes_part(t, c)) m = fmaxf(m, t);
-        }
-        red[tid] = m;
         __syncthreads();
-        for (int h = 128; h > 0; h >>= 1) {
-            if (tid < h) red[tid] = fmaxf(red[tid], red[tid + h]);
-            __syncthreads();
-        }
-        m = red[0];
-        __syncthreads();
-        // sums relative to cm = c m as rounded: exact for any reference value.  An
-        // entry more than 1000 below it adds nothing (exp is 0 from -104 on).
-        const float cm = c * m;
-        const bool inf = cm == __int_as_float(0x7f800000);
-        float z = 0.f, w = 0.f;
-        for (int64_t i = tid; i < len; i += 256) {
-            const float t = sgn * load_score(s + i);
-            if (!takes_part(t, c)) continue;
-            const float d = fmaxf(fmaf(c, t, -cm), -1000.f), p = expf(d);
-            z += p;
-            w += p * d;
-        }
-        red[tid] = z;
-        red2[tid] = w;
-        __syncthreads();
-        for (int h = 128; h > 0; h >>= 1) {
-            if (tid < h) {
-                red[tid] += red[tid + h];
-                red2[tid] += red2[tid + h];
+        for (int64_t gt = g0; gt < g1; gt += kVecs * kThreads) {
+            float t[kPer];
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) Vec<T>::unpack(raw[v], t + v * V);
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) {  // the next tile
+                const int64_t g = gt + (kVecs + v) * kThreads + tid;
+                raw[v] = g < g1 ? load_granule(x, at.len, mis, g) : make_uint4(~0u, ~0u, ~0u, ~0u);
             }
-            __syncthreads();
-        }
-        z = red[0];
-        w = red2[0];
-        __syncthreads();
-        const float logz = logf(z);  // -inf for a row with nothing left
-        if (tid == 0) {
-            a.lse[row] = inf || !(z > 0.f) ? cm : cm + logz;  // cm = -inf: nothing left
-            a.entropy[row] = inf ? __int_as_float(0x7fc00000) : z > 0.f ? logz - w / z : 0.f;
-        }
-        auto logp = [&](float t) {
-            if (!takes_part(t, c)) return __int_as_float(0xff800000);
-            if (inf) return __int_as_float(c * t == cm ? 0x7fc00000 : 0xff800000);
-            return fmaf(c, t, -cm) - logz;
-        };
-        for (int j = tid; j < a.ngiven; j += 256) {
-            const int64_t at = a.given[row * a.ngiven + j];
-            a.out_given[row * a.ngiven + j] =
-                at >= 0 && at < len ? logp(sgn * load_score(s + at)) : __int_as_float(0xff800000);
-        }
-        // key: (descending score, ascending place); ~0 for none
-        unsigned long long last = 0;
-        for (int j = 0; j < a.k; ++j) {
-            unsigned long long best = ~0ull;
-            for (int64_t i = tid; i < len; i += 256) {
-                const float t = sgn * load_score(s + i);
-                if (!takes_part(t, c)) continue;
-                const unsigned long long key =
-                    ((unsigned long long)float_key(-t) << 32) | (uint32_t)i;
-                if ((j == 0 || key > last) && key < best) best = key;
+            float m = ninf();
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+                t[u] *= sgn;
+                m = fmaxf(m, t[u]);
             }
-            redk[tid] = best;
-            __syncthreads();
-            for (int h = 128; h > 0; h >>= 1) {
-                if (tid < h) redk[tid] = min(redk[tid], redk[tid + h]);
+            const float l = c * m;
+            const bool some = l > ninf();
+            if (some) {
+                if (m > s.m) rebase(s, c, m);
+                const float cm = c * s.m;
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) {
+                    const float d = fmaxf(fmaf(c, t[u], -cm), -1000.f), e = exp_of(d);
+                    s.z += e;
+                    s.w = fmaf(e, d, s.w);
+                }
+            }
+            if (a.k > 0) {
+                int n = sm.count;  // (read by all before any can append)
+                const int able = __syncthreads_count(some && m >= tau);
+                if (able == 0) continue;
+                if (n + able * kPer > kTile / 2) {
+                    // much to append (the first tile, for one): a better bound first
+                    if (n > a.k) {
+                        n = best_of_buffer(n, a.k, sm);
+                        if (n == a.k) tau = fmaxf(tau, t_of(sm.buf[n - 1]));
+                    }
+                    tau = fmaxf(tau, offered_bound(some ? m : ninf(), a.k, sm));
+                }
+                if (some && m >= tau) {
+#pragma unroll
+                    for (int u = 0; u < kPer; ++u) {
+                        const int64_t i = (gt + (u / V) * kThreads + tid) * V - mis + u % V;
+                        if (t[u] >= tau && c * t[u] > ninf()) append(key_of(t[u], (uint32_t)i), sm);
+                    }
+                }
                 __syncthreads();
             }
-            last = redk[0];
+        }
+        s = block_join(s, c, sm);
+        int kept = 0;
+        if (a.k > 0) kept = best_of_buffer(sm.count, a.k, sm);
+        if (parts == 1) {
+            finish_row<T>(a, row, at, s, kept, c, sgn, sm);
+        } else {
+            unsigned char* o = part_at(a, unit);
+            if (tid == 0) *reinterpret_cast<float4*>(o) = make_float4(s.m, s.z, s.w, 0.f);
+            for (int j = tid; j < a.k; j += kThreads)
+                reinterpret_cast<unsigned long long*>(o + 16)[j] = j < kept ? sm.buf[j] : kNone;
             __syncthreads();
-            if (tid == 0) {
-                const int64_t at = (int64_t)(uint32_t)last;
-                a.top_index[row * a.k + j] = last == ~0ull ? -1 : at;
-                a.top[row * a.k + j] = last == ~0ull ? __int_as_float(0xff800000)
-                                                     : logp(sgn * load_score(s + at));
-            }
         }
     }
 }
 
+// Joins a row's parts: their sums in a fixed order, their best keys through the
+// same buffer.
+template <class T>
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int parts) {
+    __shared__ Shared sm;
+    const int tid = threadIdx.x;
+    const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
+    for (int64_t row = blockIdx.x; row < a.nq; row += gridDim.x) {
+        const RowAt at = row_at(a, row);
+        if (tid == 0) sm.count = 0;
+        Sums s;
+        for (int i = tid; i < parts; i += kThreads) {
+            const float4 v = *reinterpret_cast<const float4*>(part_at(a, row * parts + i));
+            Sums b;
+            b.m = v.x;
+            b.z = v.y;
+            b.w = v.z;
+            s = join(s, b, c);
+        }
+        s = block_join(s, c, sm);
+        int kept = 0;
+        if (a.k > 0) {
+            unsigned long long tau = kNone;
+            const int64_t total = (int64_t)parts * a.k;
+            for (int64_t b = 0; b < total; b += kTile) {
+                for (int64_t i = b + tid; i < min(b + kTile, total); i += kThreads) {
+                    const int p = (int)(i / a.k), j = (int)(i - (int64_t)p * a.k);
+                    const unsigned long long key = reinterpret_cast<const unsigned long long*>(
+                        part_at(a, row * parts + p) + 16)[j];
+                    append(key <= tau ? key : kNone, sm);
+                }
+                __syncthreads();
+                kept = best_of_buffer(sm.count, a.k, sm);
+                if (kept == a.k) tau = sm.buf[kept - 1];
+                __syncthreads();
+            }
+        }
+        finish_row<T>(a, row, at, s, kept, c, sgn, sm);
+    }
+}
+
+// Parts a row: enough units that the blocks the GPU holds at once (four an SM) finish
+// together, each unit worth at least a tile.  A row's fixed work (its first bound,
+// its final order) is taken as a tile.
+int parts_of(int64_t nq, int64_t n, bool ragged, int sms) {
+    const int64_t slots = 4 * (int64_t)sms;
+    const int64_t len = ragged ? n / std::max<int64_t>(nq, 1) : n;
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(len / kTile, 1), slots);
+    int best = 1;
+    double cost = 0;
+    for (int64_t p = 1; p <= most; p += 1 + p / 8) {
+        const double c = (double)((nq * p + slots - 1) / slots) * ((double)len / p + kTile);
+        if (p == 1 || c < 0.95 * cost) {
+            best = (int)p;
+            cost = c;
+        }
+        if (nq * p > 8 * slots) break;
+    }
+    return best;
+}
+
 }  // namespace
 
-int64_t score_probs_work(int64_t, int64_t, bool, int, int) { return 0; }
+int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int k, int sms) {
+    const int parts = parts_of(nq, n, ragged, sms);
+    return parts == 1 ? 0 : nq * parts * (16 + 8 * (int64_t)k);
+}
 
 cudaError_t launch_score_probs(const ProbsArgs& a, int sms, cudaStream_t st) {
-    const unsigned grid = (unsigned)std::min<int64_t>(a.nq, (int64_t)sms * 8);
-    if (a.dtype == M3G_F32)
-        score_probs_kernel<float><<<grid, 256, 0, st>>>(a);
-    else
-        score_probs_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
+    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, sms);
+    const unsigned grid = (unsigned)std::min<int64_t>(a.nq * parts, (int64_t)1 << 30);
+    const unsigned rows = (unsigned)std::min<int64_t>(a.nq, (int64_t)1 << 30);
+    if (a.dtype == M3G_F32) {
+        score_probs_kernel<float><<<grid, kThreads, 0, st>>>(a, parts);
+        if (parts > 1) join_parts_kernel<float><<<rows, kThreads, 0, st>>>(a, parts);
+    } else {
+        score_probs_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, parts);
+        if (parts > 1) join_parts_kernel<__nv_bfloat16><<<rows, kThreads, 0, st>>>(a, parts);
+    }
     return cudaGetLastError();
 }
 

@@ -553,7 +553,9 @@ def test_retrieval_with_probabilities_matches_search(R, eng):
     assert np.abs(-want_sc - top_scores)[differ].max(initial=0) <= dim * 2.0 ** -22 * 20
     assert differ.mean() < 0.02
     p = got.top.exp().sum(1)
-    assert ((p > 0) & (p <= 1 + 1e-4)).all() and (got.entropy > 0).all()
+    # (an entropy below 2^-24, one entry having nearly all of the probability, may come out as 0)
+    assert ((p > 0) & (p <= 1 + 1e-4)).all() and (got.entropy >= 0).all()
+    assert (got.entropy > 0).float().mean() > 0.5
 
 
 def test_streams_and_concurrent_calls(R, eng):
