@@ -39,10 +39,41 @@ constexpr unsigned long long kNone = ~0ull;   // no entry
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 
 struct Sums {
-    float m = -INFINITY, z = 0.f, w = 0.f;
+    float m, z, w;
 };
+__device__ __forceinline__ Sums no_sums() { return {ninf(), 0.f, 0.f}; }
 
-__device__ __forceinline__ float exp_of(float d) { return exp2f(d * 1.4426950408889634f); }
+// e^d within 2^-22 and |d| 2^-23 of its value; 0 below 2^-126
+__device__ __forceinline__ float exp_of(float d) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+    return r;
+}
+
+// Two fp32 values in one register pair: sm_100 has packed fma, mul and add.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 // a part's sums taken to another reference value
 __device__ __forceinline__ void rebase(Sums& s, float c, float m) {
@@ -220,23 +251,6 @@ struct Vec<__nv_bfloat16> {
 __device__ __forceinline__ float load_score(const float* p) { return *p; }
 __device__ __forceinline__ float load_score(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// The 16 bytes of granule g of a row whose first entry is `mis` entries into its
-// first granule; entries outside the row are NaN.
-template <class T>
-__device__ __forceinline__ uint4 load_granule(const T* row, int64_t len, int mis, int64_t g) {
-    constexpr int V = Vec<T>::kN;
-    const int64_t i = g * V - mis;
-    if (i >= 0 && i + V <= len) return __ldcs(reinterpret_cast<const uint4*>(row + i));
-    uint4 r = make_uint4(~0u, ~0u, ~0u, ~0u);  // NaNs of either type
-    if (i + V > 0 && i < len) {
-        T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-        for (int u = 0; u < V; ++u)
-            if (i + u >= 0 && i + u < len) e[u] = row[i + u];
-    }
-    return r;
-}
-
 struct RowAt {
     int64_t first, len;
 };
@@ -282,83 +296,117 @@ __device__ void finish_row(const ProbsArgs& a, int64_t row, const RowAt& at, con
     __syncthreads();
 }
 
-// A part's place in the scratch: its sums, then its best k keys.
+// A part's place in the scratch (on an 8-byte boundary): its sums, then its best k
+// keys.
 __device__ __forceinline__ unsigned char* part_at(const ProbsArgs& a, int64_t unit) {
     return static_cast<unsigned char*>(a.work) + unit * (16 + 8 * (int64_t)a.k);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 4) score_probs_kernel(ProbsArgs a, int parts) {
+__global__ void __launch_bounds__(kThreads, 3) score_probs_kernel(ProbsArgs a, int parts) {
     constexpr int V = Vec<T>::kN, kVecs = kPer / V;
     __shared__ Shared sm;
     const int tid = threadIdx.x;
     const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
+    const uint32_t flip = a.scale > 0.f ? 0u : 0x80000000u;
     for (int64_t unit = blockIdx.x; unit < a.nq * parts; unit += gridDim.x) {
         const int64_t row = unit / parts;
         const int part = (int)(unit - row * parts);
         const RowAt at = row_at(a, row);
         const T* x = static_cast<const T*>(a.scores) + at.first;
-        const int mis = (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % V);
-        const int64_t ngran = (at.len + mis + V - 1) / V;
-        const int64_t g0 = ngran * part / parts, g1 = ngran * (part + 1) / parts;
-        Sums s;
+        // the row: `head` entries up to a 16-byte boundary, whole granules of 16 bytes,
+        // the rest; a part has its share of the granules, the first one the others too
+        const int len = (int)at.len;
+        const int head = min(
+            (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)), len);
+        const int ngran = (len - head) / V;
+        const int g0 = (int)((int64_t)ngran * part / parts);
+        const int g1 = (int)((int64_t)ngran * (part + 1) / parts);
+        const uint4* gran = reinterpret_cast<const uint4*>(x + head);
+        Sums s = no_sums();
         float tau = ninf();  // entries below it are not among the best k
         if (tid == 0) sm.count = 0;
         uint4 raw[kVecs];
+        auto load = [&](int g) {
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-            const int64_t g = g0 + v * kThreads + tid;
-            raw[v] = g < g1 ? load_granule(x, at.len, mis, g) : make_uint4(~0u, ~0u, ~0u, ~0u);
-        }
-        __syncthreads();
-        for (int64_t gt = g0; gt < g1; gt += kVecs * kThreads) {
-            float t[kPer];
-#pragma unroll
-            for (int v = 0; v < kVecs; ++v) Vec<T>::unpack(raw[v], t + v * V);
-#pragma unroll
-            for (int v = 0; v < kVecs; ++v) {  // the next tile
-                const int64_t g = gt + (kVecs + v) * kThreads + tid;
-                raw[v] = g < g1 ? load_granule(x, at.len, mis, g) : make_uint4(~0u, ~0u, ~0u, ~0u);
+            for (int v = 0; v < kVecs; ++v) {
+                const int i = g + v * kThreads + tid;
+                raw[v] = i < g1 ? __ldcs(gran + i) : make_uint4(~0u, ~0u, ~0u, ~0u);  // NaNs
             }
+        };
+        load(g0);
+        __syncthreads();
+        // a tile: t[u] (NaN for none) is the row's entry place(u)
+        auto tile = [&](float(&t)[kPer], auto place) {
             float m = ninf();
 #pragma unroll
             for (int u = 0; u < kPer; ++u) {
-                t[u] *= sgn;
+                t[u] = __uint_as_float(__float_as_uint(t[u]) ^ flip);
                 m = fmaxf(m, t[u]);
             }
-            const float l = c * m;
-            const bool some = l > ninf();
+            const bool some = c * m > ninf();
             if (some) {
                 if (m > s.m) rebase(s, c, m);
                 const float cm = c * s.m;
+                const uint64_t cc = pack2(c, c), mm = pack2(-cm, -cm);
+                const uint64_t l2 = pack2(1.4426950408889634f, 1.4426950408889634f);
+                uint64_t z = 0, w = 0;
 #pragma unroll
-                for (int u = 0; u < kPer; ++u) {
-                    const float d = fmaxf(fmaf(c, t[u], -cm), -1000.f), e = exp_of(d);
-                    s.z += e;
-                    s.w = fmaf(e, d, s.w);
+                for (int u = 0; u < kPer; u += 2) {
+                    float d0, d1, e0, e1;
+                    unpack2(fma2(cc, pack2(t[u], t[u + 1]), mm), d0, d1);
+                    const uint64_t d = pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f));
+                    unpack2(mul2(d, l2), d0, d1);
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(d0));
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(d1));
+                    const uint64_t e = pack2(e0, e1);
+                    z = add2(z, e);
+                    w = fma2(e, d, w);
                 }
+                float z0, z1, w0, w1;
+                unpack2(z, z0, z1);
+                unpack2(w, w0, w1);
+                s.z += z0 + z1;
+                s.w += w0 + w1;
             }
             if (a.k > 0) {
                 int n = sm.count;  // (read by all before any can append)
                 const int able = __syncthreads_count(some && m >= tau);
-                if (able == 0) continue;
-                if (n + able * kPer > kTile / 2) {
+                if (able == 0) return;
+                if (n > 4 * a.k + 64 || n + able * kPer > kTile / 2) {
                     // much to append (the first tile, for one): a better bound first
                     if (n > a.k) {
                         n = best_of_buffer(n, a.k, sm);
                         if (n == a.k) tau = fmaxf(tau, t_of(sm.buf[n - 1]));
                     }
-                    tau = fmaxf(tau, offered_bound(some ? m : ninf(), a.k, sm));
+                    if (n + able * kPer > kTile / 2)
+                        tau = fmaxf(tau, offered_bound(some ? m : ninf(), a.k, sm));
+                    else
+                        __syncthreads();
                 }
                 if (some && m >= tau) {
 #pragma unroll
-                    for (int u = 0; u < kPer; ++u) {
-                        const int64_t i = (gt + (u / V) * kThreads + tid) * V - mis + u % V;
-                        if (t[u] >= tau && c * t[u] > ninf()) append(key_of(t[u], (uint32_t)i), sm);
-                    }
+                    for (int u = 0; u < kPer; ++u)
+                        if (t[u] >= tau && c * t[u] > ninf())
+                            append(key_of(t[u], (uint32_t)place(u)), sm);
                 }
                 __syncthreads();
             }
+        };
+        float t[kPer];
+        if (part == 0 && V * ngran < len) {  // entries outside whole granules
+            const int tail = head + V * ngran;
+            const int i = tid < head ? tid : tail + tid - head;
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) t[u] = __int_as_float(0x7fc00000);
+            if (tid < head || (tid < 2 * V && i < len)) t[0] = load_score(x + i);
+            tile(t, [&](int) { return i; });
+        }
+        for (int g = g0; g < g1; g += kVecs * kThreads) {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) Vec<T>::unpack(raw[v], t + v * V);
+            load(g + kVecs * kThreads);
+            tile(t, [&](int u) { return head + (g + (u / V) * kThreads + tid) * V + u % V; });
         }
         s = block_join(s, c, sm);
         int kept = 0;
@@ -367,7 +415,10 @@ __global__ void __launch_bounds__(kThreads, 4) score_probs_kernel(ProbsArgs a, i
             finish_row<T>(a, row, at, s, kept, c, sgn, sm);
         } else {
             unsigned char* o = part_at(a, unit);
-            if (tid == 0) *reinterpret_cast<float4*>(o) = make_float4(s.m, s.z, s.w, 0.f);
+            if (tid == 0) {
+                reinterpret_cast<float2*>(o)[0] = make_float2(s.m, s.z);
+                reinterpret_cast<float2*>(o)[1] = make_float2(s.w, 0.f);
+            }
             for (int j = tid; j < a.k; j += kThreads)
                 reinterpret_cast<unsigned long long*>(o + 16)[j] = j < kept ? sm.buf[j] : kNone;
             __syncthreads();
@@ -385,14 +436,11 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
     for (int64_t row = blockIdx.x; row < a.nq; row += gridDim.x) {
         const RowAt at = row_at(a, row);
         if (tid == 0) sm.count = 0;
-        Sums s;
+        Sums s = no_sums();
         for (int i = tid; i < parts; i += kThreads) {
-            const float4 v = *reinterpret_cast<const float4*>(part_at(a, row * parts + i));
-            Sums b;
-            b.m = v.x;
-            b.z = v.y;
-            b.w = v.z;
-            s = join(s, b, c);
+            const float2* v =
+                reinterpret_cast<const float2*>(part_at(a, row * parts + i));
+            s = join(s, Sums{v[0].x, v[0].y, v[1].x}, c);
         }
         s = block_join(s, c, sm);
         int kept = 0;
@@ -416,11 +464,11 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
     }
 }
 
-// Parts a row: enough units that the blocks the GPU holds at once (four an SM) finish
+// Parts a row: enough units that the blocks the GPU holds at once (three an SM) finish
 // together, each unit worth at least a tile.  A row's fixed work (its first bound,
 // its final order) is taken as a tile.
 int parts_of(int64_t nq, int64_t n, bool ragged, int sms) {
-    const int64_t slots = 4 * (int64_t)sms;
+    const int64_t slots = 3 * (int64_t)sms;
     const int64_t len = ragged ? n / std::max<int64_t>(nq, 1) : n;
     const int64_t most = std::min<int64_t>(std::max<int64_t>(len / kTile, 1), slots);
     int best = 1;

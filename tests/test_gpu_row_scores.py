@@ -417,7 +417,8 @@ def some_scores(nq, n, dtype, seed, ties=False):
 
 @pytest.mark.parametrize("nq,n,k", [(1, 1, 1), (1, 1, 0), (5, 2, 4), (4, 31, 32), (7, 33, 1),
                                     (3, 1000, 10), (2, 4096, 33), (6, 5001, 100), (4, 257, 128),
-                                    (1, 300001, 10), (2, 100003, 128), (300, 777, 5)])
+                                    (1, 300001, 10), (2, 100003, 128), (300, 777, 5),
+                                    (1, 50001, 1), (3, 40000, 3), (2, 70001, 33), (1, 30000, 0)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("scale", [30.0, -1.0])
 def test_score_probs(R, eng, nq, n, k, dtype, scale):
@@ -448,6 +449,28 @@ def test_score_probs_ragged(R, eng, dtype, k):
     rows = [f[a:b] for a, b in zip(off, off[1:])]
     given = torch.from_numpy(rng.integers(-1, 50, (len(size), 2))).cuda()
     probs_check(R, eng, flat, rows, 25.0, k, given, torch.from_numpy(off).cuda())
+
+
+def test_score_probs_scratch_on_any_8_byte_boundary(R, eng):
+    """Split rows of every odd and even k, the scratch 8 bytes off a 16-byte boundary, and nothing
+    written past its end."""
+    nq, n = 3, 40001
+    s = some_scores(nq, n, torch.float32, 1)
+    rows = list(s.cpu().numpy())
+    for k in (0, 1, 2, 3, 7, 127):
+        need = eng.score_probs_work(nq, n, False, k)
+        assert need > 0
+        work = torch.full((need + 64,), 0x5A, dtype=torch.uint8, device="cuda")
+        lse, ent = torch.empty(nq, device="cuda"), torch.empty(nq, device="cuda")
+        top = torch.empty(nq, max(k, 1), device="cuda")
+        idx = torch.empty(nq, max(k, 1), dtype=torch.int64, device="cuda")
+        eng.score_probs_device(s.data_ptr(), cabi.F32, nq, n, n, None, 2.0, None, 0, k,
+                               lse.data_ptr(), ent.data_ptr(), None, idx.data_ptr(),
+                               top.data_ptr(), work.data_ptr() + 8, need)
+        assert (work[:8] == 0x5A).all() and (work[8 + need:] == 0x5A).all()
+        for i, r in enumerate(probs_ref(rows, 2.0, k, None)):
+            assert close(lse[i].item(), r[0], r[5]) and close(ent[i].item(), r[1], r[6])
+            assert not k or np.array_equal(idx[i].cpu().numpy(), r[4])
 
 
 def test_score_probs_many_equal_scores(R, eng):
