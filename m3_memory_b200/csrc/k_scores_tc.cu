@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -727,9 +728,17 @@ cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* 
     constexpr size_t smem = sizeof(Smem<NT>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     auto kernel = scores_tc_kernel<F8, NT, GROUP, O>;
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // once a device (a bit each; devices past 64 set it every time)
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!(set.load() & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        set |= bit;
+    }
     CUtensorMap mx, mx32, mq;
     row_map(&mx, x, kM);
     row_map(&mx32, x, 32);

@@ -20,8 +20,11 @@ from . import cabi
 
 BLOCK = 128  # dims that share one scale
 
+_F32, _BF16, _U8, _I32, _I64 = (torch.float32, torch.bfloat16, torch.uint8, torch.int32,
+                                torch.int64)
+_DTYPES = {_F32: cabi.F32, _BF16: cabi.BF16}
 _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream, named so that the call does not wait
-_DTYPES = {torch.float32: cabi.F32, torch.bfloat16: cabi.BF16}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 class PackedRows(NamedTuple):
@@ -50,101 +53,117 @@ class ScoreProbs(NamedTuple):
     top_index: Optional[torch.Tensor]
 
 
+# The calls below are made per batch, small ones too, so their checks cost little: plain
+# comparisons, messages built only where one fails.
+
+
 def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream or _LEGACY_STREAM
+    return _raw_stream(dev) or _LEGACY_STREAM
 
 
-def _need(ok, msg):
-    if not ok:
-        raise ValueError(msg)
+def _bad(what, msg):
+    raise ValueError(f"{what} {msg}")
 
 
-def _on(t, dev, what):
-    _need(t.device == dev, f"{what} is on {t.device}, not on {dev}")
+def _device_of(t, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _bad(what, "must be a CUDA tensor")
+    return t.get_device()
 
 
 def _vector(t, dtype, n, dev, what):
-    _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and (n is None or len(t) == n),
-          f"{what} must be a contiguous {dtype} vector" + ("" if n is None else f" of {n}"))
-    _on(t, dev, what)
+    """The address of a contiguous vector of n values on the device."""
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        _bad(what, f"must be a contiguous {dtype} vector of {n}")
+    if t.get_device() != dev:
+        _bad(what, f"is on {t.device}, not on cuda:{dev}")
+    return t.data_ptr()
 
 
-def _matrix_ld(t, what):
-    """The row stride of a matrix with contiguous rows."""
-    _need(t.dim() == 2, f"{what} must be 2D")
+def _matrix(t, dev, what):
+    """(n, d, row stride) of a matrix with contiguous rows; a single row has stride d."""
+    if t.dim() != 2:
+        _bad(what, "must be 2D")
+    if t.get_device() != dev:
+        _bad(what, f"is on {t.device}, not on cuda:{dev}")
     n, d = t.shape
-    _need(d <= 1 or t.stride(1) == 1, f"{what} must have contiguous rows")
-    ld = t.stride(0) if n > 1 else max(d, t.stride(0))
-    _need(n <= 1 or ld >= d, f"{what} must not overlap itself")
-    return ld
+    ld, one = t.stride()
+    if one != 1 and d > 1:
+        _bad(what, "must have contiguous rows")
+    if n <= 1:
+        ld = d
+    elif ld < d:
+        _bad(what, "must not overlap itself")
+    return n, d, ld
 
 
 def _rows(r, dev, what):
+    """The m3g_rows of PackedRows or of a bf16 matrix."""
     if isinstance(r, PackedRows):
-        c, s = r.codes, r.scales
-        _need(c.dtype == torch.uint8 and s.dtype == torch.uint8, f"{what}: packed rows are uint8")
-        _on(c, dev, what)
-        _on(s, dev, what)
-        ld, lds = _matrix_ld(c, what), _matrix_ld(s, what)
-        n, nblk = c.shape[0], -(-r.dim // BLOCK)
-        _need(s.shape[0] == n and c.shape[1] >= r.dim > 0 and s.shape[1] >= nblk,
-              f"{what}: codes and scales do not hold {n} rows of {r.dim} dims")
-        if n == 1:  # a single row has no stride to go by
-            ld, lds = -(-max(ld, r.dim) // 16) * 16, -(-max(lds, nblk) // 4) * 4
-        return cabi.Rows(c.data_ptr(), s.data_ptr(), n, ld, lds, r.dim, cabi.E4M3)
-    _need(isinstance(r, torch.Tensor) and r.dtype == torch.bfloat16,
-          f"{what} must be PackedRows or a bf16 tensor")
-    _on(r, dev, what)
-    ld = _matrix_ld(r, what)
-    n, dim = r.shape
-    if n == 1:
-        ld = -(-max(ld, dim) // 8) * 8
+        codes, scales, dim = r
+        if codes.dtype != _U8 or scales.dtype != _U8:
+            _bad(what, "must hold uint8 codes and scales")
+        n, d, ld = _matrix(codes, dev, what)
+        ns, ds, lds = _matrix(scales, dev, what)
+        nblk = (dim + BLOCK - 1) // BLOCK
+        if ns != n or dim <= 0 or d < dim or ds < nblk:
+            _bad(what, f"codes and scales do not hold {n} rows of {dim} dims")
+        if n <= 1:  # no stride to go by
+            ld, lds = (dim + 15) // 16 * 16, (nblk + 3) // 4 * 4
+        return cabi.Rows(codes.data_ptr(), scales.data_ptr(), n, ld, lds, dim, cabi.E4M3)
+    if not isinstance(r, torch.Tensor) or r.dtype != _BF16:
+        _bad(what, "must be PackedRows or a bf16 tensor")
+    n, dim, ld = _matrix(r, dev, what)
+    if n <= 1:
+        ld = (dim + 7) // 8 * 8
     return cabi.Rows(r.data_ptr(), None, n, ld, 0, dim, cabi.BF16)
 
 
-def _out_dtype(dtype):
-    _need(dtype in _DTYPES, "scores are float32 or bfloat16")
-    return _DTYPES[dtype]
+def _dtype(t, what):
+    d = _DTYPES.get(t)
+    if d is None:
+        _bad(what, "must be float32 or bfloat16")
+    return d
 
 
-def _device(rows):
-    t = rows.codes if isinstance(rows, PackedRows) else rows
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, "rows must be on a CUDA device")
-    return t.device
+def _device(rows, what):
+    return _device_of(rows.codes if isinstance(rows, PackedRows) else rows, what)
 
 
 def pack_rows(engine, x, out=None) -> PackedRows:
     """Packs fp32 or bf16 rows ``x [n, dim]`` to 8 bits (m3g_pack_rows_device): e4m3 codes with one
     power-of-two scale per 128 dims.  ``out``: PackedRows to write instead of new ones."""
-    _need(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
-    _need(x.dtype in _DTYPES, "x must be float32 or bfloat16")
-    ldx = _matrix_ld(x, "x")
-    n, dim = x.shape
-    dev = x.device
+    dev = _device_of(x, "x")
+    dtype = _dtype(x.dtype, "x")
+    n, dim, ldx = _matrix(x, dev, "x")
     if out is None:
-        _need(dim > 0, "x has no dims")
-        nblk = -(-dim // BLOCK)
-        out = PackedRows(torch.empty((n, -(-dim // 16) * 16), dtype=torch.uint8, device=dev),
-                         torch.empty((n, -(-nblk // 4) * 4), dtype=torch.uint8, device=dev), dim)
-    _need(out.dim == dim and len(out.codes) == n, f"out does not hold {n} rows of {dim} dims")
-    engine.pack_rows_device(x.data_ptr(), _DTYPES[x.dtype], n, dim, max(ldx, dim),
-                            _rows(out, dev, "out"), _stream(dev))
+        if dim == 0:
+            _bad("x", "has no dims")
+        nblk = (dim + BLOCK - 1) // BLOCK
+        out = PackedRows(x.new_empty((n, (dim + 15) // 16 * 16), dtype=_U8),
+                         x.new_empty((n, (nblk + 3) // 4 * 4), dtype=_U8), dim)
+    elif out.dim != dim or out.codes.shape[0] != n:
+        _bad("out", f"does not hold {n} rows of {dim} dims")
+    engine.pack_rows_device(x.data_ptr(), dtype, n, dim, ldx, _rows(out, dev, "out"),
+                            _stream(dev))
     return out
 
 
 def row_scores(engine, q, x, alpha=1.0, beta=0.0, out_dtype=torch.float32, out=None):
     """``alpha * q @ x.T + beta`` for every row of q and x (m3g_row_scores_device), ``[len(q),
     len(x)]`` in float32 or bfloat16.  ``out``: a matrix to write instead of a new one."""
-    dev = _device(x)
+    dev = _device(x, "x")
     a, b = _rows(q, dev, "q"), _rows(x, dev, "x")
     if out is None:
-        out = torch.empty((a.n, b.n), dtype=out_dtype, device=dev)
+        _dtype(out_dtype, "out_dtype")
+        t = x.codes if isinstance(x, PackedRows) else x
+        out = t.new_empty((a.n, b.n), dtype=out_dtype)
         ld = b.n
     else:
-        _need(tuple(out.shape) == (a.n, b.n), f"out must be [{a.n}, {b.n}]")
-        _on(out, dev, "out")
-        ld = max(_matrix_ld(out, "out"), b.n)
-    engine.row_scores_device(a, b, alpha, beta, out.data_ptr(), _out_dtype(out.dtype), ld,
+        n, d, ld = _matrix(out, dev, "out")
+        if n != a.n or d != b.n:
+            _bad("out", f"must be [{a.n}, {b.n}]")
+    engine.row_scores_device(a, b, alpha, beta, out.data_ptr(), _dtype(out.dtype, "out"), ld,
                              _stream(dev))
     return out
 
@@ -158,21 +177,16 @@ def list_scores(engine, q, x, list_off, list_len, pair_off, out_off, out, pair_r
     ``pair_off[g] .. pair_off[g + 1]`` (int64, one entry more) probe it; pair p is row
     ``pair_row[p]`` of q (int32; row p without it, -1 for none) and writes ``list_len[g]`` scores
     from ``out[out_off[p]]`` (int64) on."""
-    dev = _device(x)
+    dev = _device(x, "x")
     a, b = _rows(q, dev, "q"), _rows(x, dev, "x")
-    ngroup, npair = len(list_off), len(out_off)
-    _vector(list_off, torch.int64, ngroup, dev, "list_off")
-    _vector(list_len, torch.int32, ngroup, dev, "list_len")
-    _vector(pair_off, torch.int64, ngroup + 1, dev, "pair_off")
-    _vector(out_off, torch.int64, npair, dev, "out_off")
-    if pair_row is not None:
-        _vector(pair_row, torch.int32, npair, dev, "pair_row")
-    _vector(out, out.dtype, None, dev, "out")
-    engine.list_scores_device(a, b, ngroup, list_off.data_ptr(), list_len.data_ptr(),
-                              pair_off.data_ptr(), npair,
-                              None if pair_row is None else pair_row.data_ptr(),
-                              out_off.data_ptr(), alpha, beta, out.data_ptr(),
-                              _out_dtype(out.dtype), len(out), _stream(dev))
+    ngroup, npair, n = list_off.numel(), out_off.numel(), out.numel()
+    engine.list_scores_device(
+        a, b, ngroup, _vector(list_off, _I64, ngroup, dev, "list_off"),
+        _vector(list_len, _I32, ngroup, dev, "list_len"),
+        _vector(pair_off, _I64, ngroup + 1, dev, "pair_off"), npair,
+        None if pair_row is None else _vector(pair_row, _I32, npair, dev, "pair_row"),
+        _vector(out_off, _I64, npair, dev, "out_off"), alpha, beta,
+        _vector(out, out.dtype, n, dev, "out"), _dtype(out.dtype, "out"), n, _stream(dev))
     return out
 
 
@@ -182,35 +196,38 @@ def score_probs(engine, scores, scale=1.0, k=0, given=None, row_off=None) -> Sco
     places in the row; -1 for none) and the k most probable entries.  Entries that are NaN, or
     -inf after scaling, are left out.  ``scores``: float32 or bfloat16 ``[nq, n]``, or a vector
     whose row i is ``scores[row_off[i]:row_off[i + 1]]`` (``row_off`` int64)."""
-    _need(isinstance(scores, torch.Tensor) and scores.is_cuda, "scores must be a CUDA tensor")
-    _need(scores.dtype in _DTYPES, "scores must be float32 or bfloat16")
-    dev = scores.device
+    dev = _device_of(scores, "scores")
+    dtype = _dtype(scores.dtype, "scores")
+    off = None
     if row_off is None:
-        ld = max(_matrix_ld(scores, "scores"), scores.shape[1])
-        nq, n = scores.shape
+        nq, n, ld = _matrix(scores, dev, "scores")
     else:
-        _vector(scores, scores.dtype, None, dev, "scores")
-        _need(len(row_off) >= 1, "row_off holds one entry more than there are rows")
-        _vector(row_off, torch.int64, None, dev, "row_off")
-        nq, n, ld = len(row_off) - 1, len(scores), 0
-    ngiven = 0
+        n, ld = scores.numel(), 0
+        nq = row_off.numel() - 1
+        if nq < 0:
+            _bad("row_off", "holds one entry more than there are rows")
+        _vector(scores, scores.dtype, n, dev, "scores")
+        off = _vector(row_off, _I64, nq + 1, dev, "row_off")
+    ngiven, given_at = 0, None
+    out_given = top = top_index = work = None
     if given is not None:
-        _need(given.dtype == torch.int64 and given.dim() == 2 and given.shape[0] == nq and
-              given.is_contiguous(), f"given must be contiguous int64 [{nq}, m]")
-        _on(given, dev, "given")
-        ngiven = given.shape[1]
-    lse = torch.empty(nq, device=dev)
-    entropy = torch.empty(nq, device=dev)
-    out_given = None if given is None else torch.empty((nq, ngiven), device=dev)
-    top = torch.empty((nq, k), device=dev) if k > 0 else None
-    top_index = torch.empty((nq, k), dtype=torch.int64, device=dev) if k > 0 else None
-    nbytes = engine.score_probs_work(nq, n, row_off is not None, k)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        if given.dtype != _I64 or not given.is_contiguous():
+            _bad("given", "must be contiguous int64")
+        g, ngiven, _ = _matrix(given, dev, "given")
+        if g != nq:
+            _bad("given", f"must have {nq} rows")
+        out_given = scores.new_empty((nq, ngiven), dtype=_F32)
+        given_at = given.data_ptr() if ngiven else None
+    lse, entropy = scores.new_empty((2, nq), dtype=_F32).unbind()
+    if k > 0:
+        top = scores.new_empty((nq, k), dtype=_F32)
+        top_index = scores.new_empty((nq, k), dtype=_I64)
+    nbytes = engine.score_probs_work(nq, n, off is not None, k)
+    if nbytes:
+        work = scores.new_empty(nbytes, dtype=_U8)
     engine.score_probs_device(
-        scores.data_ptr(), _DTYPES[scores.dtype], nq, n, ld,
-        None if row_off is None else row_off.data_ptr(), scale,
-        given.data_ptr() if ngiven else None, ngiven, k, lse.data_ptr(), entropy.data_ptr(),
-        out_given.data_ptr() if ngiven else None, top_index.data_ptr() if k > 0 else None,
-        top.data_ptr() if k > 0 else None, work.data_ptr() if nbytes else None, nbytes,
-        _stream(dev))
+        scores.data_ptr(), dtype, nq, n, ld, off, scale, given_at, ngiven, k, lse.data_ptr(),
+        entropy.data_ptr(), out_given.data_ptr() if ngiven else None,
+        top_index.data_ptr() if k > 0 else None, top.data_ptr() if k > 0 else None,
+        work.data_ptr() if nbytes else None, nbytes, _stream(dev))
     return ScoreProbs(lse, entropy, out_given, top, top_index)
