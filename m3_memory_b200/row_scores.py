@@ -24,7 +24,11 @@ _F32, _BF16, _U8, _I32, _I64 = (torch.float32, torch.bfloat16, torch.uint8, torc
                                 torch.int64)
 _DTYPES = {_F32: cabi.F32, _BF16: cabi.BF16}
 _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream, named so that the call does not wait
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:  # a torch without CUDA, or without this short cut
+    def _raw_stream(dev):
+        return torch.cuda.current_stream(dev).cuda_stream
 
 
 class PackedRows(NamedTuple):
