@@ -415,7 +415,7 @@ int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, 
  * A l of +inf gives logsumexp +inf and entropy NaN.  d_work holds work_bytes >=
  * m3g_score_probs_work() bytes on an 8-byte boundary (null where that is 0): scratch
  * of this call, which calls that overlap must not share. */
-int m3g_score_probs_work(m3g_engine* e, int64_t nq, int64_t n, int ragged, int k,
+int m3g_score_probs_work(m3g_engine* e, int64_t nq, int64_t n, int ragged, int dtype, int k,
                          int64_t* out_bytes);
 int m3g_score_probs_device(m3g_engine* e, const void* d_scores, int dtype, int64_t nq, int64_t n,
                            int64_t ld, const int64_t* d_row_off, float scale,

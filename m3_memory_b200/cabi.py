@@ -122,7 +122,7 @@ SIGNATURES = {
     "m3g_list_scores_device": (_i32, [_vp, ct.POINTER(Rows), ct.POINTER(Rows), _i64, _vp, _vp,
                                       _vp, _i64, _vp, _vp, ct.c_float, ct.c_float, _vp, _i32,
                                       _i64, _vp]),
-    "m3g_score_probs_work": (_i32, [_vp, _i64, _i64, _i32, _i32, _pi64]),
+    "m3g_score_probs_work": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _pi64]),
     "m3g_score_probs_device": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _vp, ct.c_float, _vp,
                                       _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "m3g_set_profiling": (_i32, [_vp, _i32]),
@@ -493,9 +493,9 @@ class Engine:
                                            pair_off_ptr, npair, pair_row_ptr, out_off_ptr, alpha,
                                            beta, out_ptr, out_dtype, out_n, stream))
 
-    def score_probs_work(self, nq, n, ragged, k):
+    def score_probs_work(self, nq, n, ragged, dtype, k):
         out = ct.c_int64()
-        check(lib().m3g_score_probs_work(self.h, nq, n, int(ragged), k, ct.byref(out)))
+        check(lib().m3g_score_probs_work(self.h, nq, n, int(ragged), dtype, k, ct.byref(out)))
         return out.value
 
     def score_probs_device(self, scores_ptr, dtype, nq, n, ld, row_off_ptr, scale, given_ptr,

@@ -534,12 +534,12 @@ int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, 
     });
 }
 
-int m3g_score_probs_work(m3g_engine* e, int64_t nq, int64_t n, int ragged, int k,
+int m3g_score_probs_work(m3g_engine* e, int64_t nq, int64_t n, int ragged, int dtype, int k,
                          int64_t* out_bytes) {
     M3G_ENGINE_OR_FAIL(e);
     return guarded([&] {
         if (!out_bytes) m3g::fail(M3G_EINVAL, "score_probs_work: out missing");
-        *out_bytes = e->eng.score_probs_work(nq, n, ragged != 0, k);
+        *out_bytes = e->eng.score_probs_work(nq, n, ragged != 0, dtype, k);
     });
 }
 

@@ -9,32 +9,43 @@
 // exactly whatever that rounding was.  Entries that are NaN, or -inf after scaling,
 // come out of max(d, -1000) with e^d = 0.
 //
-// The best k of a row pass through a buffer in shared memory: a thread offers the
-// entries of its 16 that reach the current bound tau, a lower bound of the k-th
-// best.  tau first comes from the threads' own maxima (at least k of them reach the
-// smallest of the warps' ceil(k / 8)-th largest), later from the buffer itself, which
-// is cut to its best k when it could overflow.
+// A warp takes a row, or one of P parts of it where rows are few, on its own: no warp
+// waits for another, and one's latencies (row offsets, the final order, the outputs)
+// pass behind the others' work.  Its scores come through a ring of three 4 KB bulk
+// copies, so 144 KB an SM are in flight whatever the warps do.  Parts leave (m, z, w)
+// and their best k in the caller's scratch and a second kernel joins them.
 //
-// The scores' bytes bound it.  A block of 256 threads takes a row, or one of P parts
-// of it where rows are few; parts leave (m, z, w) and their best k in the caller's
-// scratch and a second kernel joins them.
+// The best k pass through a buffer of the warp's: entries that reach the bound tau, a
+// lower bound of the k-th best.  tau first comes from the maxima of a stage's granules
+// (16 bytes, eight a lane): at least k of the 256 reach the smallest of the eight
+// rounds' ceil(k / 8)-th largest.  The buffer is cut to its best k, which sharpens tau,
+// whenever it holds twice as many, and before it could overflow.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "common.cuh"
 #include "kernels_scores.h"
+#include "tc.cuh"
+#include "topk.cuh"
 
 namespace m3g {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kPer = 16;                      // entries a thread holds of a tile
-constexpr int kTile = kThreads * kPer;
-constexpr int kBuf = kTile + kProbsMaxK;      // a tile always fits behind the best k
 constexpr unsigned long long kNone = ~0ull;   // no entry
+
+// the warps of the first kernel
+constexpr int kWarps = 12;
+constexpr int kStages = 3, kStageBytes = 4096, kRounds = kStageBytes / 512;
+constexpr int kCap = kProbsMaxK + 512;  // a round (32 granules of up to 8) fits behind k
+
+// the block that joins a row's parts
+constexpr int kThreads = 256, kJoinWarps = kThreads / 32;
+constexpr int kTile = 4096;
+constexpr int kBuf = kTile + kProbsMaxK;
 
 __device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
 
@@ -95,34 +106,17 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
     return a;
 }
 
-struct Shared {
-    unsigned long long buf[kBuf], best[kProbsMaxK];
-    Sums sums[kWarps];
-    float offer[kWarps];
-    int count;
-};
-
-// One value for each warp, the sums of all its lanes in fixed order.
+// The sums of all lanes, in fixed order, in every lane.
 __device__ __forceinline__ Sums warp_join(Sums s, float c) {
+    float m = s.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    rebase(s, c, m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        Sums b;
-        b.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-        b.z = __shfl_xor_sync(0xffffffffu, s.z, o);
-        b.w = __shfl_xor_sync(0xffffffffu, s.w, o);
-        s = join(s, b, c);
+        s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+        s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
     }
-    return s;
-}
-
-__device__ __forceinline__ Sums block_join(Sums s, float c, Shared& sm) {
-    s = warp_join(s, c);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm.sums[threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = sm.sums[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) s = join(s, sm.sums[i], c);
     return s;
 }
 
@@ -139,26 +133,44 @@ __device__ __forceinline__ float warp_sort_desc(float v) {
     return v;
 }
 
-// A value that at least k of the threads' v reach (all of them if fewer than k are
-// above -inf): the smallest of the warps' ceil(k / kWarps)-th largest.
-__device__ __forceinline__ float offered_bound(float v, int k, Shared& sm) {
-    v = warp_sort_desc(v);
-    const int nth = (k + kWarps - 1) / kWarps - 1;
-    if ((threadIdx.x & 31) == nth) sm.offer[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float b = sm.offer[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) b = fminf(b, sm.offer[i]);
-    __syncthreads();
-    return b;
-}
-
 // Keys order entries best first: descending t, then ascending place.
 __device__ __forceinline__ unsigned long long key_of(float t, uint32_t place) {
     return ((unsigned long long)float_key(-t) << 32) | place;
 }
 __device__ __forceinline__ float t_of(unsigned long long key) {
     return -key_float((uint32_t)(key >> 32));
+}
+
+struct Shared {  // of the joining block
+    unsigned long long buf[kBuf], best[kProbsMaxK];
+    Sums sums[kJoinWarps];
+    float offer[kJoinWarps];
+    int count;
+};
+
+__device__ __forceinline__ Sums block_join(Sums s, float c, Shared& sm) {
+    s = warp_join(s, c);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm.sums[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = sm.sums[0];
+#pragma unroll
+    for (int i = 1; i < kJoinWarps; ++i) s = join(s, sm.sums[i], c);
+    return s;
+}
+
+// A value that at least k of the threads' v reach (all of them if fewer than k are
+// above -inf): the smallest of the warps' ceil(k / 8)-th largest.
+__device__ __forceinline__ float offered_bound(float v, int k, Shared& sm) {
+    v = warp_sort_desc(v);
+    const int nth = (k + kJoinWarps - 1) / kJoinWarps - 1;
+    if ((threadIdx.x & 31) == nth) sm.offer[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float b = sm.offer[0];
+#pragma unroll
+    for (int i = 1; i < kJoinWarps; ++i) b = fminf(b, sm.offer[i]);
+    __syncthreads();
+    return b;
 }
 
 // Appends the keys a thread passes (any of them kNone) to the buffer.
@@ -188,11 +200,12 @@ __device__ __noinline__ int best_of_buffer(int n, int k, Shared& sm) {
         } else {
             __syncthreads();
             sm.buf[tid] = best;
+            if (tid == 0) sm.buf[kThreads] = kNone;
             __syncthreads();
             int better = 0;
             for (int i = 0; i < kThreads; ++i) better += sm.buf[i] < best;
-            // (n > kThreads, so every thread has a best one and they are distinct)
-            if (better == k - 1) sm.buf[kThreads] = best;
+            __syncthreads();
+            if (best != kNone && better == k - 1) sm.buf[kThreads] = best;
             __syncthreads();
             bound = sm.buf[kThreads];
         }
@@ -208,6 +221,8 @@ __device__ __noinline__ int best_of_buffer(int n, int k, Shared& sm) {
     }
     // places among the n entries that are left
     const int kept = min(n, k);
+    if (tid < kProbsMaxK) sm.best[tid] = kNone;
+    __syncthreads();
     for (int i0 = tid; i0 < n; i0 += kThreads) {
         const unsigned long long key = sm.buf[i0];
         int better = 0;
@@ -269,31 +284,32 @@ __device__ __forceinline__ float log_prob(float t, float c, float cm, float logz
     return fmaf(c, t, -cm) - logz;
 }
 
-// The answer of a row from its sums and its best entries (in sm.buf, sorted).
+// The answer of a row from its sums and its best entries (keys, sorted, kept of them),
+// by `threads` threads.
 template <class T>
-__device__ void finish_row(const ProbsArgs& a, int64_t row, const RowAt& at, const Sums& s,
-                           int kept, float c, float sgn, Shared& sm) {
-    const float cm = s.z > 0.f || s.m > ninf() ? c * s.m : ninf();
+__device__ __forceinline__ void finish_row(const ProbsArgs& a, int64_t row, const RowAt& at,
+                                           const Sums& s, const unsigned long long* keys,
+                                           int kept, float c, float sgn, int tid, int threads) {
+    const float cm = s.m > ninf() ? c * s.m : ninf();
     const bool inf = cm == __int_as_float(0x7f800000);
     const float logz = logf(s.z);
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         a.lse[row] = inf || !(s.z > 0.f) ? cm : cm + logz;
         a.entropy[row] = inf          ? __int_as_float(0x7fc00000)
                          : s.z > 0.f ? fmaxf(logz - s.w / s.z, 0.f)  // (roundings aside)
                                      : 0.f;
     }
     const T* x = static_cast<const T*>(a.scores) + at.first;
-    for (int j = threadIdx.x; j < a.ngiven; j += kThreads) {
+    for (int j = tid; j < a.ngiven; j += threads) {
         const int64_t g = a.given[row * a.ngiven + j];
         a.out_given[row * a.ngiven + j] =
             g >= 0 && g < at.len ? log_prob(sgn * load_score(x + g), c, cm, logz) : ninf();
     }
-    for (int j = threadIdx.x; j < a.k; j += kThreads) {
-        const unsigned long long key = j < kept ? sm.buf[j] : kNone;
+    for (int j = tid; j < a.k; j += threads) {
+        const unsigned long long key = j < kept ? keys[j] : kNone;
         a.top_index[row * a.k + j] = key == kNone ? -1 : (int64_t)(uint32_t)key;
         a.top[row * a.k + j] = key == kNone ? ninf() : log_prob(t_of(key), c, cm, logz);
     }
-    __syncthreads();
 }
 
 // A part's place in the scratch (on an 8-byte boundary): its sums, then its best k
@@ -302,132 +318,350 @@ __device__ __forceinline__ unsigned char* part_at(const ProbsArgs& a, int64_t un
     return static_cast<unsigned char*>(a.work) + unit * (16 + 8 * (int64_t)a.k);
 }
 
+// ---------------- the warps ----------------
+
+struct alignas(128) WarpShared {
+    unsigned char stage[kStages][kStageBytes];
+    unsigned long long buf[kCap];
+    uint64_t full[kStages];
+    int count;
+    int lost;  // a wait gave up
+};
+
+// The number of the buffer's n keys whose high (or, among those whose high word is
+// `high`, low) word is at most v.
+__device__ __forceinline__ int count_to(const unsigned long long* buf, int n, uint32_t v, bool low,
+                                        uint32_t high) {
+    int c = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const uint32_t h = (uint32_t)(buf[i] >> 32);
+        c += low ? h < high || (h == high && (uint32_t)buf[i] <= v) : h <= v;
+    }
+    return __reduce_add_sync(0xffffffffu, c);
+}
+
+// Cuts the warp's buffer of n keys to its best min(k, n), sorted; returns their number.
+// Keys past the 32 KW that the sort holds are dropped first, by bisection on the high
+// words and, where entries tie, on the low ones (their places).
+template <int KW>
+__device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    if (n > 32 * KW) {
+        uint32_t lo = 0xFFFFFFFFu, hi = 0;
+        for (int i = lane; i < n; i += 32) {
+            lo = min(lo, (uint32_t)(buf[i] >> 32));
+            hi = max(hi, (uint32_t)(buf[i] >> 32));
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        int c = n;  // keys up to hi
+        while (c > 32 * KW && lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int m = count_to(buf, n, mid, false, 0);
+            if (m >= k) {
+                hi = mid;
+                c = m;
+            } else {
+                lo = mid + 1;
+            }
+        }
+        const uint32_t high = hi;
+        uint32_t low = 0xFFFFFFFFu;
+        if (c > 32 * KW) {  // hi is the one high word at the k-th place: the lowest of its places
+            uint32_t a = 0, b = 0xFFFFFFFFu;
+            while (c > 32 * KW) {
+                const uint32_t mid = a + (b - a) / 2;
+                const int m = count_to(buf, n, mid, true, high);
+                if (m >= k) {
+                    b = mid;
+                    c = m;
+                } else {
+                    a = mid + 1;
+                }
+            }
+            low = b;
+        }
+        const unsigned long long last = ((unsigned long long)high << 32) | low;
+        int m = 0;
+        for (int b = 0; b < n; b += 32) {
+            const unsigned long long key = b + lane < n ? buf[b + lane] : kNone;
+            const bool keep = b + lane < n && key <= last;
+            const unsigned ball = __ballot_sync(0xffffffffu, keep);
+            if (keep) buf[m + __popc(ball & ((1u << lane) - 1u))] = key;  // (at or before b + lane)
+            m += __popc(ball);
+            __syncwarp();
+        }
+        n = m;
+    }
+    // bitonic sort of 32 KW keys, key 32 r + lane in v[r]
+    unsigned long long v[KW];
+#pragma unroll
+    for (int r = 0; r < KW; ++r) v[r] = 32 * r + lane < n ? buf[32 * r + lane] : kNone;
+#pragma unroll
+    for (int size = 2; size <= 32 * KW; size <<= 1)
+#pragma unroll
+        for (int j = size >> 1; j > 0; j >>= 1) {
+            if (j >= 32) {
+#pragma unroll
+                for (int r = 0; r < KW; ++r) {
+                    const int o = r ^ (j >> 5);
+                    if (o > r) {
+                        const bool up = ((32 * r) & size) == 0;
+                        const unsigned long long a = min(v[r], v[o]), b = max(v[r], v[o]);
+                        v[r] = up ? a : b;
+                        v[o] = up ? b : a;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < KW; ++r) {
+                    const unsigned long long p = shfl_xor_u64(v[r], j);
+                    const bool up = ((32 * r + lane) & size) == 0, lower = (lane & j) == 0;
+                    v[r] = lower == up ? min(v[r], p) : max(v[r], p);
+                }
+            }
+        }
+    n = min(n, k);
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < KW; ++r)
+        if (32 * r + lane < n) buf[32 * r + lane] = v[r];
+    __syncwarp();
+    return n;
+}
+
+// A warp's unit: a row's part p of P.  The row: `head` entries up to a 16-byte
+// boundary, whole granules of 16 bytes, the rest; a part has its share of the
+// granules, the first one the other entries too.
 template <class T>
-__global__ void __launch_bounds__(kThreads, 3) score_probs_kernel(ProbsArgs a, int parts) {
-    constexpr int V = Vec<T>::kN, kVecs = kPer / V;
-    __shared__ Shared sm;
-    const int tid = threadIdx.x;
+struct Unit {
+    int64_t row;
+    RowAt at;
+    int head, ngran, g0, g1, part;
+
+    __device__ __forceinline__ void set(const ProbsArgs& a, int64_t unit, int parts, RowAt r) {
+        constexpr int V = Vec<T>::kN;
+        row = unit / parts;
+        part = (int)(unit - row * parts);
+        at = r;
+        const uintptr_t x =
+            reinterpret_cast<uintptr_t>(static_cast<const T*>(a.scores) + at.first);
+        head = min((int)((16 - (x & 15)) % 16 / sizeof(T)), (int)at.len);
+        ngran = ((int)at.len - head) / V;
+        g0 = (int)((int64_t)ngran * part / parts);
+        g1 = (int)((int64_t)ngran * (part + 1) / parts);
+    }
+    __device__ __forceinline__ const T* base(const ProbsArgs& a) const {
+        return static_cast<const T*>(a.scores) + at.first;
+    }
+};
+
+template <class T, int KW>
+__global__ void __launch_bounds__(kWarps * 32, 1)
+    score_probs_kernel(ProbsArgs a, int parts, int* err) {
+    constexpr int V = Vec<T>::kN;
+    extern __shared__ unsigned char smem_raw[];
+    const int lane = threadIdx.x & 31;
+    WarpShared& sm = reinterpret_cast<WarpShared*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127))[threadIdx.x >> 5];
     const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
     const uint32_t flip = a.scale > 0.f ? 0u : 0x80000000u;
-    for (int64_t unit = blockIdx.x; unit < a.nq * parts; unit += gridDim.x) {
-        const int64_t row = unit / parts;
-        const int part = (int)(unit - row * parts);
-        const RowAt at = row_at(a, row);
-        const T* x = static_cast<const T*>(a.scores) + at.first;
-        // the row: `head` entries up to a 16-byte boundary, whole granules of 16 bytes,
-        // the rest; a part has its share of the granules, the first one the others too
-        const int len = (int)at.len;
-        const int head = min(
-            (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)), len);
-        const int ngran = (len - head) / V;
-        const int g0 = (int)((int64_t)ngran * part / parts);
-        const int g1 = (int)((int64_t)ngran * (part + 1) / parts);
-        const uint4* gran = reinterpret_cast<const uint4*>(x + head);
+    const int64_t units = a.nq * parts, step = (int64_t)gridDim.x * kWarps;
+    // a block's warps take units far apart, so that a few units use every SM
+    const int64_t first = (int64_t)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+    if (lane == 0) {
+        for (int s = 0; s < kStages; ++s) mbar_init(&sm.full[s], 1);
+        fence_mbar_init();
+        sm.lost = 0;
+    }
+    __syncwarp();
+    bool lost = false;  // a wait gave up: nothing more is read or written
+
+    // the copies run ahead of the work by up to kStages, into later units too
+    Unit<T> load;
+    int64_t load_unit = first;
+    RowAt load_next = {0, 0};  // the row after it, fetched early
+    int load_g = 0;
+    uint32_t issued = 0, used = 0;
+    auto row_of = [&](int64_t unit) {
+        return unit < units ? row_at(a, unit / parts) : RowAt{0, 0};
+    };
+    auto open_load = [&](RowAt r) {
+        if (load_unit < units) {
+            load.set(a, load_unit, parts, r);
+            load_g = load.g0;
+            load_next = row_of(load_unit + step);
+        }
+    };
+    auto issue = [&] {
+        while (issued - used < kStages && load_unit < units) {
+            if (load_g >= load.g1) {
+                load_unit += step;
+                open_load(load_next);
+                continue;
+            }
+            const int n = min(load.g1 - load_g, kStageBytes / 16);
+            const uint32_t s = issued % kStages;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&sm.full[s], (uint32_t)n * 16);
+                bulk_g2s(sm.stage[s], load.base(a) + load.head + (int64_t)load_g * V,
+                         (uint32_t)n * 16, &sm.full[s]);
+            }
+            load_g += n;
+            ++issued;
+        }
+    };
+    open_load(row_of(load_unit));
+    issue();
+
+    RowAt next_row = row_of(first);
+    for (int64_t unit = first; unit < units && !lost; unit += step) {
+        Unit<T> u;
+        u.set(a, unit, parts, next_row);
+        next_row = row_of(unit + step);
+        const T* x = u.base(a);
+        const int len = (int)u.at.len;
+        // the entries outside whole granules, one a lane, used last
+        float edge = __int_as_float(0x7fc00000);
+        const int edge_at = lane < u.head ? lane : u.head + V * u.ngran + lane - u.head;
+        if (u.part == 0 && edge_at < len && (lane < u.head || edge_at >= u.head + V * u.ngran))
+            edge = load_score(x + edge_at);
         Sums s = no_sums();
         float tau = ninf();  // entries below it are not among the best k
-        if (tid == 0) sm.count = 0;
-        uint4 raw[kVecs];
-        auto load = [&](int g) {
-#pragma unroll
-            for (int v = 0; v < kVecs; ++v) {
-                const int i = g + v * kThreads + tid;
-                raw[v] = i < g1 ? __ldcs(gran + i) : make_uint4(~0u, ~0u, ~0u, ~0u);  // NaNs
-            }
+        int n = 0;           // keys in the buffer
+        auto sharpen = [&] {
+            n = cut<KW>(sm.buf, n, a.k);
+            if (n == a.k) tau = fmaxf(tau, t_of(sm.buf[n - 1]));
         };
-        load(g0);
-        __syncthreads();
-        // a tile: t[u] (NaN for none) is the row's entry place(u)
-        auto tile = [&](float(&t)[kPer], auto place) {
-            float m = ninf();
-#pragma unroll
-            for (int u = 0; u < kPer; ++u) {
-                t[u] = __uint_as_float(__float_as_uint(t[u]) ^ flip);
-                m = fmaxf(m, t[u]);
+        // Appends the entries of a lane that reach tau, E of them from t, if `some`.
+        auto offer = [&](const float* t, int E, bool some, int place) {
+            const unsigned ball = __ballot_sync(0xffffffffu, some);
+            if (!ball) return;
+            if (n + __popc(ball) * E > kCap) sharpen();
+            if (lane == 0) sm.count = n;
+            __syncwarp();
+            if (some)
+                for (int i = 0; i < E; ++i)
+                    if (t[i] >= tau && c * t[i] > ninf())
+                        sm.buf[atomicAdd(&sm.count, 1)] = key_of(t[i], (uint32_t)(place + i));
+            __syncwarp();
+            n = sm.count;
+            __syncwarp();
+        };
+        for (int g = u.g0; g < u.g1; g += kStageBytes / 16) {
+            const uint32_t slot = used % kStages;
+            const bool ok = mbar_wait(&sm.full[slot], (used / kStages) & 1u, &sm.lost);
+            if (!__all_sync(0xffffffffu, ok)) {
+                lost = true;
+                break;
             }
-            const bool some = c * m > ninf();
-            if (some) {
+            const uint4* st = reinterpret_cast<const uint4*>(sm.stage[slot]);
+            const int left = u.g1 - g;  // granules
+            float m = ninf(), top[kRounds];
+            float t[kRounds][V];
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const uint4 nan = make_uint4(~0u, ~0u, ~0u, ~0u);
+                Vec<T>::unpack(r * 32 + lane < left ? st[r * 32 + lane] : nan, t[r]);
+                top[r] = ninf();
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    t[r][i] = __uint_as_float(__float_as_uint(t[r][i]) ^ flip);
+                    top[r] = fmaxf(top[r], t[r][i]);
+                }
+                m = fmaxf(m, top[r]);
+            }
+            __syncwarp();
+            ++used;
+            issue();  // the stage is in registers: its slot is free
+            if (c * m > ninf()) {
                 if (m > s.m) rebase(s, c, m);
                 const float cm = c * s.m;
                 const uint64_t cc = pack2(c, c), mm = pack2(-cm, -cm);
                 const uint64_t l2 = pack2(1.4426950408889634f, 1.4426950408889634f);
                 uint64_t z = 0, w = 0;
 #pragma unroll
-                for (int u = 0; u < kPer; u += 2) {
-                    float d0, d1, e0, e1;
-                    unpack2(fma2(cc, pack2(t[u], t[u + 1]), mm), d0, d1);
-                    const uint64_t d = pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f));
-                    unpack2(mul2(d, l2), d0, d1);
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(d0));
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(d1));
-                    const uint64_t e = pack2(e0, e1);
-                    z = add2(z, e);
-                    w = fma2(e, d, w);
-                }
+                for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) {
+                        float d0, d1, e0, e1;
+                        unpack2(fma2(cc, pack2(t[r][i], t[r][i + 1]), mm), d0, d1);
+                        const uint64_t d = pack2(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f));
+                        unpack2(mul2(d, l2), d0, d1);
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(d0));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(d1));
+                        const uint64_t e = pack2(e0, e1);
+                        z = add2(z, e);
+                        w = fma2(e, d, w);
+                    }
                 float z0, z1, w0, w1;
                 unpack2(z, z0, z1);
                 unpack2(w, w0, w1);
                 s.z += z0 + z1;
                 s.w += w0 + w1;
             }
-            if (a.k > 0) {
-                int n = sm.count;  // (read by all before any can append)
-                const int able = __syncthreads_count(some && m >= tau);
-                if (able == 0) return;
-                if (n > 4 * a.k + 64 || n + able * kPer > kTile / 2) {
-                    // much to append (the first tile, for one): a better bound first
-                    if (n > a.k) {
-                        n = best_of_buffer(n, a.k, sm);
-                        if (n == a.k) tau = fmaxf(tau, t_of(sm.buf[n - 1]));
+            if (a.k > 0 && __any_sync(0xffffffffu, m >= tau && c * m > ninf())) {
+                if (g == u.g0) {
+                    if (KW == 1) {
+                        tau = __shfl_sync(0xffffffffu, warp_sort_desc(m), a.k - 1);
+                    } else {
+                        const int nth = (a.k + kRounds - 1) / kRounds - 1;
+                        float b = __int_as_float(0x7f800000);
+#pragma unroll
+                        for (int r = 0; r < kRounds; ++r)
+                            b = fminf(b, __shfl_sync(0xffffffffu, warp_sort_desc(top[r]), nth));
+                        tau = b;
                     }
-                    if (n + able * kPer > kTile / 2)
-                        tau = fmaxf(tau, offered_bound(some ? m : ninf(), a.k, sm));
-                    else
-                        __syncthreads();
                 }
-                if (some && m >= tau) {
 #pragma unroll
-                    for (int u = 0; u < kPer; ++u)
-                        if (t[u] >= tau && c * t[u] > ninf())
-                            append(key_of(t[u], (uint32_t)place(u)), sm);
-                }
-                __syncthreads();
+                for (int r = 0; r < kRounds; ++r)
+                    offer(t[r], V, top[r] >= tau && c * top[r] > ninf(),
+                          u.head + (g + r * 32 + lane) * V);
+                if (n >= 2 * a.k) sharpen();
             }
-        };
-        float t[kPer];
-        if (part == 0 && V * ngran < len) {  // entries outside whole granules
-            const int tail = head + V * ngran;
-            const int i = tid < head ? tid : tail + tid - head;
-#pragma unroll
-            for (int u = 0; u < kPer; ++u) t[u] = __int_as_float(0x7fc00000);
-            if (tid < head || (tid < 2 * V && i < len)) t[0] = load_score(x + i);
-            tile(t, [&](int) { return i; });
         }
-        for (int g = g0; g < g1; g += kVecs * kThreads) {
-#pragma unroll
-            for (int v = 0; v < kVecs; ++v) Vec<T>::unpack(raw[v], t + v * V);
-            load(g + kVecs * kThreads);
-            tile(t, [&](int u) { return head + (g + (u / V) * kThreads + tid) * V + u % V; });
+        if (lost) break;
+        if (__any_sync(0xffffffffu, edge == edge)) {
+            float t[1] = {__uint_as_float(__float_as_uint(edge) ^ flip)};
+            const bool some = c * t[0] > ninf();
+            if (some) {
+                if (t[0] > s.m) rebase(s, c, t[0]);
+                const float d = fmaxf(fmaf(c, t[0], -(c * s.m)), -1000.f), e = exp_of(d);
+                s.z += e;
+                s.w = fmaf(e, d, s.w);
+            }
+            if (a.k > 0) offer(t, 1, some && t[0] >= tau, edge_at);
         }
-        s = block_join(s, c, sm);
+        s = warp_join(s, c);
         int kept = 0;
-        if (a.k > 0) kept = best_of_buffer(sm.count, a.k, sm);
+        if (a.k > 0) kept = cut<KW>(sm.buf, n, a.k);
         if (parts == 1) {
-            finish_row<T>(a, row, at, s, kept, c, sgn, sm);
+            finish_row<T>(a, u.row, u.at, s, sm.buf, kept, c, sgn, lane, 32);
         } else {
             unsigned char* o = part_at(a, unit);
-            if (tid == 0) {
+            if (lane == 0) {
                 reinterpret_cast<float2*>(o)[0] = make_float2(s.m, s.z);
                 reinterpret_cast<float2*>(o)[1] = make_float2(s.w, 0.f);
             }
-            for (int j = tid; j < a.k; j += kThreads)
+            for (int j = lane; j < a.k; j += 32)
                 reinterpret_cast<unsigned long long*>(o + 16)[j] = j < kept ? sm.buf[j] : kNone;
-            __syncthreads();
         }
+        __syncwarp();
+    }
+    if (lost) {
+        // no copy may still be landing when the warp leaves
+        if (lane == 0) {
+            atomicOr(err + kScoreTimeout, 1);
+            for (uint32_t k = used; k != issued; ++k)
+                mbar_drain(&sm.full[k % kStages], (k / kStages) & 1u);
+        }
+        __syncwarp();
     }
 }
 
 // Joins a row's parts: their sums in a fixed order, their best keys through the
-// same buffer.
+// block's buffer.
 template <class T>
 __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int parts) {
     __shared__ Shared sm;
@@ -435,46 +669,40 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
     const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
     for (int64_t row = blockIdx.x; row < a.nq; row += gridDim.x) {
         const RowAt at = row_at(a, row);
-        if (tid == 0) sm.count = 0;
         Sums s = no_sums();
         for (int i = tid; i < parts; i += kThreads) {
-            const float2* v =
-                reinterpret_cast<const float2*>(part_at(a, row * parts + i));
+            const float2* v = reinterpret_cast<const float2*>(part_at(a, row * parts + i));
             s = join(s, Sums{v[0].x, v[0].y, v[1].x}, c);
         }
-        s = block_join(s, c, sm);
         int kept = 0;
-        if (a.k > 0) {
-            unsigned long long tau = kNone;
-            const int64_t total = (int64_t)parts * a.k;
-            for (int64_t b = 0; b < total; b += kTile) {
-                for (int64_t i = b + tid; i < min(b + kTile, total); i += kThreads) {
-                    const int p = (int)(i / a.k), j = (int)(i - (int64_t)p * a.k);
-                    const unsigned long long key = reinterpret_cast<const unsigned long long*>(
-                        part_at(a, row * parts + p) + 16)[j];
-                    append(key <= tau ? key : kNone, sm);
-                }
-                __syncthreads();
-                kept = best_of_buffer(sm.count, a.k, sm);
-                if (kept == a.k) tau = sm.buf[kept - 1];
-                __syncthreads();
+        const int total = parts * a.k;
+        for (int b = 0; b < total; b += kTile) {
+            const int n = min(kTile, total - b);
+            for (int i = tid; i < n; i += kThreads) {
+                const int p = (b + i) / a.k, j = (b + i) - p * a.k;
+                sm.buf[kept + i] = reinterpret_cast<const unsigned long long*>(
+                    part_at(a, row * parts + p) + 16)[j];
             }
+            __syncthreads();
+            kept = best_of_buffer(kept + n, a.k, sm);
         }
-        finish_row<T>(a, row, at, s, kept, c, sgn, sm);
+        s = block_join(s, c, sm);
+        finish_row<T>(a, row, at, s, sm.buf, kept, c, sgn, tid, kThreads);
+        __syncthreads();
     }
 }
 
-// Parts a row: enough units that the blocks the GPU holds at once (three an SM) finish
-// together, each unit worth at least a tile.  A row's fixed work (its first bound,
-// its final order) is taken as a tile.
-int parts_of(int64_t nq, int64_t n, bool ragged, int sms) {
-    const int64_t slots = 3 * (int64_t)sms;
+// Parts a row: enough units for the GPU's warps to finish together, each worth at least
+// four stages.  A unit's fixed work (its first bound, its final order) is taken as one
+// stage.
+int parts_of(int64_t nq, int64_t n, bool ragged, int esize, int sms) {
+    const int64_t slots = (int64_t)kWarps * sms, stage = kStageBytes / esize;
     const int64_t len = ragged ? n / std::max<int64_t>(nq, 1) : n;
-    const int64_t most = std::min<int64_t>(std::max<int64_t>(len / kTile, 1), slots);
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(len / (4 * stage), 1), slots);
     int best = 1;
     double cost = 0;
     for (int64_t p = 1; p <= most; p += 1 + p / 8) {
-        const double c = (double)((nq * p + slots - 1) / slots) * ((double)len / p + kTile);
+        const double c = (double)((nq * p + slots - 1) / slots) * ((double)len / p + stage);
         if (p == 1 || c < 0.95 * cost) {
             best = (int)p;
             cost = c;
@@ -484,25 +712,45 @@ int parts_of(int64_t nq, int64_t n, bool ragged, int sms) {
     return best;
 }
 
+template <class T, int KW>
+cudaError_t launch_kw(const ProbsArgs& a, int parts, int* err, int sms, cudaStream_t st) {
+    constexpr int smem = (int)sizeof(WarpShared) * kWarps + 128;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    static std::atomic<uint64_t> set{0};  // a bit a device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!(set.load() & bit)) {
+        e = cudaFuncSetAttribute(score_probs_kernel<T, KW>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        set |= bit;
+    }
+    const unsigned grid = (unsigned)std::min<int64_t>(a.nq * parts, sms);
+    score_probs_kernel<T, KW><<<grid, kWarps * 32, smem, st>>>(a, parts, err);
+    if (parts > 1)
+        join_parts_kernel<T><<<(unsigned)std::min<int64_t>(a.nq, 1 << 30), kThreads, 0, st>>>(
+            a, parts);
+    return cudaGetLastError();
+}
+
+int element_size(int dtype) { return dtype == M3G_F32 ? 4 : 2; }
+
 }  // namespace
 
-int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int k, int sms) {
-    const int parts = parts_of(nq, n, ragged, sms);
+int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, int sms) {
+    const int parts = parts_of(nq, n, ragged, element_size(dtype), sms);
     return parts == 1 ? 0 : nq * parts * (16 + 8 * (int64_t)k);
 }
 
-cudaError_t launch_score_probs(const ProbsArgs& a, int sms, cudaStream_t st) {
-    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, sms);
-    const unsigned grid = (unsigned)std::min<int64_t>(a.nq * parts, (int64_t)1 << 30);
-    const unsigned rows = (unsigned)std::min<int64_t>(a.nq, (int64_t)1 << 30);
-    if (a.dtype == M3G_F32) {
-        score_probs_kernel<float><<<grid, kThreads, 0, st>>>(a, parts);
-        if (parts > 1) join_parts_kernel<float><<<rows, kThreads, 0, st>>>(a, parts);
-    } else {
-        score_probs_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, parts);
-        if (parts > 1) join_parts_kernel<__nv_bfloat16><<<rows, kThreads, 0, st>>>(a, parts);
-    }
-    return cudaGetLastError();
+cudaError_t launch_score_probs(const ProbsArgs& a, int* err, int sms, cudaStream_t st) {
+    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, element_size(a.dtype), sms);
+    if (a.dtype == M3G_F32)
+        return a.k <= 32 ? launch_kw<float, 1>(a, parts, err, sms, st)
+                         : launch_kw<float, 4>(a, parts, err, sms, st);
+    return a.k <= 32 ? launch_kw<__nv_bfloat16, 1>(a, parts, err, sms, st)
+                     : launch_kw<__nv_bfloat16, 4>(a, parts, err, sms, st);
 }
 
 }  // namespace m3g

@@ -35,7 +35,7 @@ cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const Score
                                int sms, cudaStream_t st);
 
 constexpr int kProbsMaxK = 128;
-int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int k, int sms);
+int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, int sms);
 struct ProbsArgs {
     const void* scores;
     int dtype;
@@ -49,6 +49,6 @@ struct ProbsArgs {
     float* top;
     void* work;
 };
-cudaError_t launch_score_probs(const ProbsArgs& a, int sms, cudaStream_t st);
+cudaError_t launch_score_probs(const ProbsArgs& a, int* err, int sms, cudaStream_t st);
 
 }  // namespace m3g

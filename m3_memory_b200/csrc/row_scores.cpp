@@ -131,9 +131,11 @@ void Engine::list_scores(const m3g_rows* q, const m3g_rows* x, const ScoreGroups
     if (!ext) row_score_errors();
 }
 
-int64_t Engine::score_probs_work(int64_t nq, int64_t n, bool ragged, int k) {
+int64_t Engine::score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k) {
+    if (dtype != M3G_F32 && dtype != M3G_BF16)
+        fail(M3G_EINVAL, "score_probs_work: scores are fp32 or bf16");
     if (nq < 0 || n < 0 || k < 0) fail(M3G_EINVAL, "score_probs_work: bad sizes");
-    return m3g::score_probs_work(nq, n, ragged, k, num_sms_);
+    return m3g::score_probs_work(nq, n, ragged, dtype, k, num_sms_);
 }
 
 void Engine::score_probs(const ProbsArgs& a, int64_t work_bytes, cudaStream_t ext) {
@@ -158,13 +160,13 @@ void Engine::score_probs(const ProbsArgs& a, int64_t work_bytes, cudaStream_t ex
         !aligned(a.given, 8) || !aligned(a.top_index, 8) || !aligned(a.lse, 4) ||
         !aligned(a.entropy, 4) || !aligned(a.out_given, 4) || !aligned(a.top, 4))
         fail(M3G_EINVAL, "score_probs: misaligned buffers");
-    const int64_t need = score_probs_work(a.nq, a.n, a.row_off != nullptr, a.k);
+    const int64_t need = score_probs_work(a.nq, a.n, a.row_off != nullptr, a.dtype, a.k);
     if (need > 0 && (!a.work || work_bytes < need || !aligned(a.work, 8)))
         fail(M3G_EINVAL, "score_probs: work needs " + std::to_string(need) +
                              " bytes on an 8-byte boundary");
     DeviceGuard g(device_);
-    M3G_CK(launch_score_probs(a, num_sms_, ext));
-    if (!ext) M3G_CK(cudaStreamSynchronize(ext));
+    M3G_CK(launch_score_probs(a, score_err(), num_sms_, ext));
+    if (!ext) row_score_errors();
 }
 
 }  // namespace m3g

@@ -226,7 +226,7 @@ def score_probs(engine, scores, scale=1.0, k=0, given=None, row_off=None) -> Sco
     if k > 0:
         top = scores.new_empty((nq, k), dtype=_F32)
         top_index = scores.new_empty((nq, k), dtype=_I64)
-    nbytes = engine.score_probs_work(nq, n, off is not None, k)
+    nbytes = engine.score_probs_work(nq, n, off is not None, dtype, k)
     if nbytes:
         work = scores.new_empty(nbytes, dtype=_U8)
     engine.score_probs_device(

@@ -458,7 +458,7 @@ def test_score_probs_scratch_on_any_8_byte_boundary(R, eng):
     s = some_scores(nq, n, torch.float32, 1)
     rows = list(s.cpu().numpy())
     for k in (0, 1, 2, 3, 7, 127):
-        need = eng.score_probs_work(nq, n, False, k)
+        need = eng.score_probs_work(nq, n, False, cabi.F32, k)
         assert need > 0
         work = torch.full((need + 64,), 0x5A, dtype=torch.uint8, device="cuda")
         lse, ent = torch.empty(nq, device="cuda"), torch.empty(nq, device="cuda")

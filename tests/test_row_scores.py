@@ -64,7 +64,7 @@ def test_null_rows_and_null_engine(eng):
     assert L.m3g_row_scores_device(None, ct.byref(rows()), ct.byref(rows()), 1.0, 0.0, P, 0, 8,
                                    None) == cabi.M3G_EINVAL
     assert L.m3g_pack_rows_device(eng.h, P, 0, 8, 200, 200, None, None) == cabi.M3G_EINVAL
-    assert L.m3g_score_probs_work(eng.h, 1, 1, 0, 0, None) == cabi.M3G_EINVAL
+    assert L.m3g_score_probs_work(eng.h, 1, 1, 0, 0, 0, None) == cabi.M3G_EINVAL
 
 
 @pytest.mark.parametrize("case", [
