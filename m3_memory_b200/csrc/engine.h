@@ -261,7 +261,7 @@ class Engine {
     void list_scores(const m3g_rows* q, const m3g_rows* x, const ScoreGroups& groups, float alpha,
                      float beta, void* d_out, int out_dtype, cudaStream_t ext_stream);
     int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k);
-    void score_probs(const ProbsArgs& a, int64_t work_bytes, cudaStream_t ext_stream);
+    void score_probs(ProbsArgs a, int64_t work_bytes, cudaStream_t ext_stream);
 
     void info(int index_id, int* dim, int* metric, int* normalized, int* nlist);
     void cluster_size(int index_id, int cid, int64_t* size, int64_t* live);

@@ -7,7 +7,7 @@
 // w' = e^(c m - c M) (w + (c m - c M) z); then logsumexp = c M + log z and
 // entropy = log z - w / z.  d is one fma on c m as rounded, so the formulas hold
 // exactly whatever that rounding was.  Entries that are NaN, or -inf after scaling,
-// come out of max(d, -1000) with e^d = 0.
+// come out of max(d, -1000) with e^d = 0; a.lowest is the least t that is neither.
 //
 // A warp takes a row, or one of P parts of it where rows are few, on its own: no warp
 // waits for another, and one's latencies (row offsets, the final order, the outputs)
@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels_scores.h"
@@ -37,10 +38,12 @@ namespace {
 
 constexpr unsigned long long kNone = ~0ull;   // no entry
 
-// the warps of the first kernel
-constexpr int kWarps = 12;
-constexpr int kStages = 3, kStageBytes = 4096, kRounds = kStageBytes / 512;
-constexpr int kCap = kProbsMaxK + 512;  // a round (32 granules of up to 8) fits behind k
+// The warps of the first kernel, as many as shared memory holds: their latencies, not
+// the bytes, are what the best k cost.  KW: k <= 32 KW.
+constexpr int kStages = 2, kStageBytes = 4096, kRounds = kStageBytes / 512;
+constexpr __host__ __device__ int warps_of(int kw) { return kw == 1 ? 20 : 16; }
+// keys a warp's buffer holds: fewer than 2 k + 8, and a round (32 granules of up to 8)
+constexpr __host__ __device__ int cap_of(int kw) { return 64 * kw + 32 + 256; }
 
 // the block that joins a row's parts
 constexpr int kThreads = 256, kJoinWarps = kThreads / 32;
@@ -320,45 +323,50 @@ __device__ __forceinline__ unsigned char* part_at(const ProbsArgs& a, int64_t un
 
 // ---------------- the warps ----------------
 
+template <int KW>
 struct alignas(128) WarpShared {
     unsigned char stage[kStages][kStageBytes];
-    unsigned long long buf[kCap];
+    unsigned long long buf[cap_of(KW)];
     uint64_t full[kStages];
-    int count;
     int lost;  // a wait gave up
 };
 
-// The number of the buffer's n keys whose high (or, among those whose high word is
-// `high`, low) word is at most v.
-__device__ __forceinline__ int count_to(const unsigned long long* buf, int n, uint32_t v, bool low,
-                                        uint32_t high) {
+// The number of all lanes' words that are at most v.
+template <int W>
+__device__ __forceinline__ int count_to(const uint32_t (&w)[W], uint32_t v) {
     int c = 0;
-    for (int i = threadIdx.x & 31; i < n; i += 32) {
-        const uint32_t h = (uint32_t)(buf[i] >> 32);
-        c += low ? h < high || (h == high && (uint32_t)buf[i] <= v) : h <= v;
-    }
+#pragma unroll
+    for (int r = 0; r < W; ++r) c += w[r] <= v;
     return __reduce_add_sync(0xffffffffu, c);
 }
 
 // Cuts the warp's buffer of n keys to its best min(k, n), sorted; returns their number.
 // Keys past the 32 KW that the sort holds are dropped first, by bisection on the high
-// words and, where entries tie, on the low ones (their places).
+// words for one that at least k and at most 32 KW keys reach and, where more than those
+// share the k-th place's high word, on the low ones (their places).
 template <int KW>
 __device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
+    constexpr int W = cap_of(KW) / 32;
     const int lane = threadIdx.x & 31;
     __syncwarp();
     if (n > 32 * KW) {
-        uint32_t lo = 0xFFFFFFFFu, hi = 0;
-        for (int i = lane; i < n; i += 32) {
-            lo = min(lo, (uint32_t)(buf[i] >> 32));
-            hi = max(hi, (uint32_t)(buf[i] >> 32));
+        // (no key's high word is ~0: that is where float_key puts NaN)
+        uint32_t w[W], lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+        for (int r = 0; r < W; ++r) {
+            w[r] = 0xFFFFFFFFu;
+            if (32 * r + lane < n) {
+                w[r] = (uint32_t)(buf[32 * r + lane] >> 32);
+                lo = min(lo, w[r]);
+                hi = max(hi, w[r]);
+            }
         }
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
         int c = n;  // keys up to hi
         while (c > 32 * KW && lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2;
-            const int m = count_to(buf, n, mid, false, 0);
+            const int m = count_to(w, mid);
             if (m >= k) {
                 hi = mid;
                 c = m;
@@ -368,11 +376,18 @@ __device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
         }
         const uint32_t high = hi;
         uint32_t low = 0xFFFFFFFFu;
-        if (c > 32 * KW) {  // hi is the one high word at the k-th place: the lowest of its places
-            uint32_t a = 0, b = 0xFFFFFFFFu;
+        if (c > 32 * KW) {
+            // places, plus one, of the keys of that high word; 0 for those before it
+#pragma unroll
+            for (int r = 0; r < W; ++r)
+                if (32 * r + lane < n)
+                    w[r] = w[r] < high    ? 0u
+                           : w[r] == high ? (uint32_t)buf[32 * r + lane] + 1u
+                                          : 0xFFFFFFFFu;
+            uint32_t a = 0, b = 0xFFFFFFFEu;  // (places are below 2^31)
             while (c > 32 * KW) {
                 const uint32_t mid = a + (b - a) / 2;
-                const int m = count_to(buf, n, mid, true, high);
+                const int m = count_to(w, mid);
                 if (m >= k) {
                     b = mid;
                     c = m;
@@ -380,10 +395,11 @@ __device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
                     a = mid + 1;
                 }
             }
-            low = b;
+            low = b - 1u;
         }
         const unsigned long long last = ((unsigned long long)high << 32) | low;
         int m = 0;
+#pragma unroll 1
         for (int b = 0; b < n; b += 32) {
             const unsigned long long key = b + lane < n ? buf[b + lane] : kNone;
             const bool keep = b + lane < n && key <= last;
@@ -401,10 +417,10 @@ __device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
 #pragma unroll
     for (int size = 2; size <= 32 * KW; size <<= 1)
 #pragma unroll
-        for (int j = size >> 1; j > 0; j >>= 1) {
-            if (j >= 32) {
+        for (int j = size >> 1; j > 0; j >>= 1)
 #pragma unroll
-                for (int r = 0; r < KW; ++r) {
+            for (int r = 0; r < KW; ++r) {
+                if (j >= 32) {
                     const int o = r ^ (j >> 5);
                     if (o > r) {
                         const bool up = ((32 * r) & size) == 0;
@@ -412,16 +428,12 @@ __device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
                         v[r] = up ? a : b;
                         v[o] = up ? b : a;
                     }
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < KW; ++r) {
+                } else {
                     const unsigned long long p = shfl_xor_u64(v[r], j);
                     const bool up = ((32 * r + lane) & size) == 0, lower = (lane & j) == 0;
                     v[r] = lower == up ? min(v[r], p) : max(v[r], p);
                 }
             }
-        }
     n = min(n, k);
     __syncwarp();
 #pragma unroll
@@ -458,16 +470,16 @@ struct Unit {
 };
 
 template <class T, int KW>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(warps_of(KW) * 32, 1)
     score_probs_kernel(ProbsArgs a, int parts, int* err) {
     constexpr int V = Vec<T>::kN;
     extern __shared__ unsigned char smem_raw[];
     const int lane = threadIdx.x & 31;
-    WarpShared& sm = reinterpret_cast<WarpShared*>(
+    WarpShared<KW>& sm = reinterpret_cast<WarpShared<KW>*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127))[threadIdx.x >> 5];
     const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
     const uint32_t flip = a.scale > 0.f ? 0u : 0x80000000u;
-    const int64_t units = a.nq * parts, step = (int64_t)gridDim.x * kWarps;
+    const int64_t units = a.nq * parts, step = (int64_t)gridDim.x * warps_of(KW);
     // a block's warps take units far apart, so that a few units use every SM
     const int64_t first = (int64_t)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
     if (lane == 0) {
@@ -528,26 +540,25 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         if (u.part == 0 && edge_at < len && (lane < u.head || edge_at >= u.head + V * u.ngran))
             edge = load_score(x + edge_at);
         Sums s = no_sums();
-        float tau = ninf();  // entries below it are not among the best k
+        float tau = a.lowest;  // entries below it are not among the best k
         int n = 0;           // keys in the buffer
         auto sharpen = [&] {
             n = cut<KW>(sm.buf, n, a.k);
             if (n == a.k) tau = fmaxf(tau, t_of(sm.buf[n - 1]));
         };
-        // Appends the entries of a lane that reach tau, E of them from t, if `some`.
-        auto offer = [&](const float* t, int E, bool some, int place) {
-            const unsigned ball = __ballot_sync(0xffffffffu, some);
-            if (!ball) return;
-            if (n + __popc(ball) * E > kCap) sharpen();
-            if (lane == 0) sm.count = n;
-            __syncwarp();
-            if (some)
-                for (int i = 0; i < E; ++i)
-                    if (t[i] >= tau && c * t[i] > ninf())
-                        sm.buf[atomicAdd(&sm.count, 1)] = key_of(t[i], (uint32_t)(place + i));
-            __syncwarp();
-            n = sm.count;
-            __syncwarp();
+        // Appends the lanes' entries (E each) that reach tau.
+        auto offer = [&](const auto& t, int place) {
+            constexpr int E = sizeof(t) / sizeof(float);
+            if (n + 32 * E > cap_of(KW)) sharpen();
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const bool hit = t[i] >= tau;
+                const unsigned ball = __ballot_sync(0xffffffffu, hit);
+                if (hit)
+                    sm.buf[n + __popc(ball & ((1u << lane) - 1u))] =
+                        key_of(t[i], (uint32_t)(place + i));
+                n += __popc(ball);
+            }
         };
         for (int g = u.g0; g < u.g1; g += kStageBytes / 16) {
             const uint32_t slot = used % kStages;
@@ -558,31 +569,36 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
             }
             const uint4* st = reinterpret_cast<const uint4*>(sm.stage[slot]);
             const int left = u.g1 - g;  // granules
-            float m = ninf(), top[kRounds];
-            float t[kRounds][V];
-#pragma unroll
-            for (int r = 0; r < kRounds; ++r) {
+            // the lane's granule of round r, oriented, NaN past the last one
+            auto granule = [&](int r, float(&v)[V]) {
                 const uint4 nan = make_uint4(~0u, ~0u, ~0u, ~0u);
-                Vec<T>::unpack(r * 32 + lane < left ? st[r * 32 + lane] : nan, t[r]);
+                Vec<T>::unpack(r * 32 + lane < left ? st[r * 32 + lane] : nan, v);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    v[i] = __uint_as_float(__float_as_uint(v[i]) ^ flip);
+            };
+            // the sums, half of the stage's entries at a time in registers
+            float m = ninf(), top[kRounds];
+            auto half = [&](auto from) {
+            constexpr int R0 = decltype(from)::value, R1 = R0 + kRounds / 2;
+            float t[kRounds / 2][V], hm = ninf();
+#pragma unroll
+            for (int r = R0; r < R1; ++r) {
+                granule(r, t[r - R0]);
                 top[r] = ninf();
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    t[r][i] = __uint_as_float(__float_as_uint(t[r][i]) ^ flip);
-                    top[r] = fmaxf(top[r], t[r][i]);
-                }
-                m = fmaxf(m, top[r]);
+                for (int i = 0; i < V; ++i) top[r] = fmaxf(top[r], t[r - R0][i]);
+                hm = fmaxf(hm, top[r]);
             }
-            __syncwarp();
-            ++used;
-            issue();  // the stage is in registers: its slot is free
-            if (c * m > ninf()) {
-                if (m > s.m) rebase(s, c, m);
+            m = fmaxf(m, hm);
+            if (hm >= a.lowest) {
+                if (hm > s.m) rebase(s, c, hm);
                 const float cm = c * s.m;
                 const uint64_t cc = pack2(c, c), mm = pack2(-cm, -cm);
                 const uint64_t l2 = pack2(1.4426950408889634f, 1.4426950408889634f);
                 uint64_t z = 0, w = 0;
 #pragma unroll
-                for (int r = 0; r < kRounds; ++r)
+                for (int r = 0; r < kRounds / 2; ++r)
 #pragma unroll
                     for (int i = 0; i < V; i += 2) {
                         float d0, d1, e0, e1;
@@ -601,37 +617,55 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
                 s.z += z0 + z1;
                 s.w += w0 + w1;
             }
-            if (a.k > 0 && __any_sync(0xffffffffu, m >= tau && c * m > ninf())) {
+            };
+            half(std::integral_constant<int, 0>());
+            half(std::integral_constant<int, kRounds / 2>());
+            if (a.k > 0 && __any_sync(0xffffffffu, m >= tau)) {
                 if (g == u.g0) {
                     if (KW == 1) {
-                        tau = __shfl_sync(0xffffffffu, warp_sort_desc(m), a.k - 1);
+                        tau = fmaxf(tau, __shfl_sync(0xffffffffu, warp_sort_desc(m), a.k - 1));
                     } else {
                         const int nth = (a.k + kRounds - 1) / kRounds - 1;
                         float b = __int_as_float(0x7f800000);
+#pragma unroll 1
+                        for (int r = 0; r < kRounds; ++r) {
+                            float v[V], best = ninf();
+                            granule(r, v);
 #pragma unroll
-                        for (int r = 0; r < kRounds; ++r)
-                            b = fminf(b, __shfl_sync(0xffffffffu, warp_sort_desc(top[r]), nth));
-                        tau = b;
+                            for (int i = 0; i < V; ++i) best = fmaxf(best, v[i]);
+                            b = fminf(b, __shfl_sync(0xffffffffu, warp_sort_desc(best), nth));
+                        }
+                        tau = fmaxf(tau, b);
                     }
                 }
+                unsigned act = 0;
 #pragma unroll
                 for (int r = 0; r < kRounds; ++r)
-                    offer(t[r], V, top[r] >= tau && c * top[r] > ninf(),
-                          u.head + (g + r * 32 + lane) * V);
-                if (n >= 2 * a.k) sharpen();
+                    act |= __any_sync(0xffffffffu, top[r] >= tau) ? 1u << r : 0u;
+                // (read again, round by round, in a short loop)
+#pragma unroll 1
+                for (; act; act &= act - 1) {
+                    const int r = __ffs(act) - 1;
+                    float v[V];
+                    granule(r, v);
+                    offer(v, u.head + (g + r * 32 + lane) * V);
+                }
+                if (n >= 2 * a.k + 8) sharpen();
             }
+            __syncwarp();
+            ++used;
+            issue();
         }
         if (lost) break;
         if (__any_sync(0xffffffffu, edge == edge)) {
-            float t[1] = {__uint_as_float(__float_as_uint(edge) ^ flip)};
-            const bool some = c * t[0] > ninf();
-            if (some) {
+            const float t[1] = {__uint_as_float(__float_as_uint(edge) ^ flip)};
+            if (t[0] >= a.lowest) {
                 if (t[0] > s.m) rebase(s, c, t[0]);
                 const float d = fmaxf(fmaf(c, t[0], -(c * s.m)), -1000.f), e = exp_of(d);
                 s.z += e;
                 s.w = fmaf(e, d, s.w);
             }
-            if (a.k > 0) offer(t, 1, some && t[0] >= tau, edge_at);
+            if (a.k > 0) offer(t, edge_at);
         }
         s = warp_join(s, c);
         int kept = 0;
@@ -695,8 +729,8 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
 // Parts a row: enough units for the GPU's warps to finish together, each worth at least
 // four stages.  A unit's fixed work (its first bound, its final order) is taken as one
 // stage.
-int parts_of(int64_t nq, int64_t n, bool ragged, int esize, int sms) {
-    const int64_t slots = (int64_t)kWarps * sms, stage = kStageBytes / esize;
+int parts_of(int64_t nq, int64_t n, bool ragged, int esize, int k, int sms) {
+    const int64_t slots = (int64_t)warps_of(k <= 32 ? 1 : 4) * sms, stage = kStageBytes / esize;
     const int64_t len = ragged ? n / std::max<int64_t>(nq, 1) : n;
     const int64_t most = std::min<int64_t>(std::max<int64_t>(len / (4 * stage), 1), slots);
     int best = 1;
@@ -714,7 +748,7 @@ int parts_of(int64_t nq, int64_t n, bool ragged, int esize, int sms) {
 
 template <class T, int KW>
 cudaError_t launch_kw(const ProbsArgs& a, int parts, int* err, int sms, cudaStream_t st) {
-    constexpr int smem = (int)sizeof(WarpShared) * kWarps + 128;
+    constexpr int smem = (int)sizeof(WarpShared<KW>) * warps_of(KW) + 128;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     static std::atomic<uint64_t> set{0};  // a bit a device
     int dev = 0;
@@ -728,7 +762,7 @@ cudaError_t launch_kw(const ProbsArgs& a, int parts, int* err, int sms, cudaStre
         set |= bit;
     }
     const unsigned grid = (unsigned)std::min<int64_t>(a.nq * parts, sms);
-    score_probs_kernel<T, KW><<<grid, kWarps * 32, smem, st>>>(a, parts, err);
+    score_probs_kernel<T, KW><<<grid, warps_of(KW) * 32, smem, st>>>(a, parts, err);
     if (parts > 1)
         join_parts_kernel<T><<<(unsigned)std::min<int64_t>(a.nq, 1 << 30), kThreads, 0, st>>>(
             a, parts);
@@ -740,12 +774,12 @@ int element_size(int dtype) { return dtype == M3G_F32 ? 4 : 2; }
 }  // namespace
 
 int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, int sms) {
-    const int parts = parts_of(nq, n, ragged, element_size(dtype), sms);
+    const int parts = parts_of(nq, n, ragged, element_size(dtype), k, sms);
     return parts == 1 ? 0 : nq * parts * (16 + 8 * (int64_t)k);
 }
 
 cudaError_t launch_score_probs(const ProbsArgs& a, int* err, int sms, cudaStream_t st) {
-    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, element_size(a.dtype), sms);
+    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, element_size(a.dtype), a.k, sms);
     if (a.dtype == M3G_F32)
         return a.k <= 32 ? launch_kw<float, 1>(a, parts, err, sms, st)
                          : launch_kw<float, 4>(a, parts, err, sms, st);

@@ -42,6 +42,7 @@ struct ProbsArgs {
     int64_t nq, n, ld;
     const int64_t* row_off;
     float scale;
+    float lowest;  // the least oriented score whose product with |scale| is not -inf
     const int64_t* given;
     int ngiven, k;
     float *lse, *entropy, *out_given;

@@ -53,6 +53,16 @@ void check_out(const char* who, const void* out, int out_dtype) {
         fail(M3G_EINVAL, std::string(who) + ": output missing or misaligned");
 }
 
+// The least t with c * t > -inf in fp32 (c > 0): -FLT_MAX, or about -FLT_MAX / c.
+float lowest_score(float c) {
+    const float most = std::numeric_limits<float>::max(), none = -INFINITY;
+    volatile float p;  // rounded to fp32
+    float t = c <= 1.f ? -most : -most / c;
+    while (p = c * t, p == none) t = std::nextafter(t, 0.f);
+    while (t > -most && (p = c * std::nextafter(t, none), p != none)) t = std::nextafter(t, none);
+    return t;
+}
+
 }  // namespace
 
 int* Engine::score_err() {
@@ -138,7 +148,7 @@ int64_t Engine::score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, 
     return m3g::score_probs_work(nq, n, ragged, dtype, k, num_sms_);
 }
 
-void Engine::score_probs(const ProbsArgs& a, int64_t work_bytes, cudaStream_t ext) {
+void Engine::score_probs(ProbsArgs a, int64_t work_bytes, cudaStream_t ext) {
     if (a.dtype != M3G_F32 && a.dtype != M3G_BF16)
         fail(M3G_EINVAL, "score_probs: scores are fp32 or bf16");
     if (a.nq < 0 || a.n < 0 || a.ngiven < 0 || a.k < 0)
@@ -165,6 +175,7 @@ void Engine::score_probs(const ProbsArgs& a, int64_t work_bytes, cudaStream_t ex
         fail(M3G_EINVAL, "score_probs: work needs " + std::to_string(need) +
                              " bytes on an 8-byte boundary");
     DeviceGuard g(device_);
+    a.lowest = lowest_score(std::fabs(a.scale));
     M3G_CK(launch_score_probs(a, score_err(), num_sms_, ext));
     if (!ext) row_score_errors();
 }
