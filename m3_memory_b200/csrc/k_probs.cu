@@ -694,6 +694,10 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
     }
 }
 
+// The sums and keys of the first kernel, visible to one launched to start before its
+// end.
+__device__ __forceinline__ void after_first_kernel() { cudaGridDependencySynchronize(); }
+
 // Joins a row's parts: their sums in a fixed order, their best keys through the
 // block's buffer.
 template <class T>
@@ -701,6 +705,7 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
     __shared__ Shared sm;
     const int tid = threadIdx.x;
     const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
+    after_first_kernel();
     for (int64_t row = blockIdx.x; row < a.nq; row += gridDim.x) {
         const RowAt at = row_at(a, row);
         Sums s = no_sums();
@@ -726,24 +731,62 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
     }
 }
 
-// Parts a row: enough units for the GPU's warps to finish together, each worth at least
-// four stages.  A unit's fixed work (its first bound, its final order) is taken as one
-// stage.
-int parts_of(int64_t nq, int64_t n, bool ragged, int esize, int k, int sms) {
-    const int64_t slots = (int64_t)warps_of(k <= 32 ? 1 : 4) * sms, stage = kStageBytes / esize;
-    const int64_t len = ragged ? n / std::max<int64_t>(nq, 1) : n;
-    const int64_t most = std::min<int64_t>(std::max<int64_t>(len / (4 * stage), 1), slots);
-    int best = 1;
-    double cost = 0;
-    for (int64_t p = 1; p <= most; p += 1 + p / 8) {
-        const double c = (double)((nq * p + slots - 1) / slots) * ((double)len / p + stage);
-        if (p == 1 || c < 0.95 * cost) {
-            best = (int)p;
-            cost = c;
+// The same by a warp a row, where all the parts' keys fit a warp's buffer.
+template <class T, int KW>
+__global__ void __launch_bounds__(128) join_few_parts_kernel(ProbsArgs a, int parts) {
+    __shared__ unsigned long long bufs[4][cap_of(KW)];
+    const int lane = threadIdx.x & 31;
+    unsigned long long* buf = bufs[threadIdx.x >> 5];
+    const float c = fabsf(a.scale), sgn = a.scale > 0.f ? 1.f : -1.f;
+    after_first_kernel();
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); row < a.nq;
+         row += (int64_t)gridDim.x * 4) {
+        const RowAt at = row_at(a, row);
+        Sums s = no_sums();
+        for (int i = lane; i < parts; i += 32) {
+            const float2* v = reinterpret_cast<const float2*>(part_at(a, row * parts + i));
+            s = join(s, Sums{v[0].x, v[0].y, v[1].x}, c);
         }
-        if (nq * p > 8 * slots) break;
+        int n = 0;
+        for (int b = 0; b < parts * a.k; b += 32) {
+            const int i = b + lane, p = i / max(a.k, 1);
+            const unsigned long long key =
+                i < parts * a.k ? reinterpret_cast<const unsigned long long*>(
+                                      part_at(a, row * parts + p) + 16)[i - p * a.k]
+                                : kNone;
+            const unsigned ball = __ballot_sync(0xffffffffu, key != kNone);
+            if (key != kNone) buf[n + __popc(ball & ((1u << lane) - 1u))] = key;
+            n += __popc(ball);
+        }
+        s = warp_join(s, c);
+        const int kept = a.k > 0 ? cut<KW>(buf, n, a.k) : 0;
+        finish_row<T>(a, row, at, s, buf, kept, c, sgn, lane, 32);
+        __syncwarp();
     }
-    return best;
+}
+
+// Parts a row: twelve units an SM are enough warps to keep the copies in flight (with
+// fewer, larger ones less of the work on the best k); none shorter than two stages.
+int parts_of(int64_t nq, int64_t n, bool ragged, int esize, int sms) {
+    const int64_t len = ragged ? n / std::max<int64_t>(nq, 1) : n;
+    const int64_t want = (12 * (int64_t)sms + nq - 1) / std::max<int64_t>(nq, 1);
+    return (int)std::max<int64_t>(std::min(want, len / (2 * kStageBytes / esize)), 1);
+}
+
+// A kernel that may start before the one before it on the stream has ended.
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, cudaStream_t st,
+                         A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <class T, int KW>
@@ -763,10 +806,12 @@ cudaError_t launch_kw(const ProbsArgs& a, int parts, int* err, int sms, cudaStre
     }
     const unsigned grid = (unsigned)std::min<int64_t>(a.nq * parts, sms);
     score_probs_kernel<T, KW><<<grid, warps_of(KW) * 32, smem, st>>>(a, parts, err);
-    if (parts > 1)
-        join_parts_kernel<T><<<(unsigned)std::min<int64_t>(a.nq, 1 << 30), kThreads, 0, st>>>(
-            a, parts);
-    return cudaGetLastError();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || parts == 1) return e;
+    if ((int64_t)parts * a.k <= cap_of(KW) && parts <= 256)
+        return launch_after(join_few_parts_kernel<T, KW>, (unsigned)((a.nq + 3) / 4), 128, st, a,
+                            parts);
+    return launch_after(join_parts_kernel<T>, (unsigned)a.nq, kThreads, st, a, parts);
 }
 
 int element_size(int dtype) { return dtype == M3G_F32 ? 4 : 2; }
@@ -774,12 +819,12 @@ int element_size(int dtype) { return dtype == M3G_F32 ? 4 : 2; }
 }  // namespace
 
 int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, int sms) {
-    const int parts = parts_of(nq, n, ragged, element_size(dtype), k, sms);
+    const int parts = parts_of(nq, n, ragged, element_size(dtype), sms);
     return parts == 1 ? 0 : nq * parts * (16 + 8 * (int64_t)k);
 }
 
 cudaError_t launch_score_probs(const ProbsArgs& a, int* err, int sms, cudaStream_t st) {
-    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, element_size(a.dtype), a.k, sms);
+    const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, element_size(a.dtype), sms);
     if (a.dtype == M3G_F32)
         return a.k <= 32 ? launch_kw<float, 1>(a, parts, err, sms, st)
                          : launch_kw<float, 4>(a, parts, err, sms, st);
