@@ -343,11 +343,15 @@ __device__ __forceinline__ int count_to(const uint32_t (&w)[W], uint32_t v) {
 // Cuts the warp's buffer of n keys to its best min(k, n), sorted; returns their number.
 // Keys past the 32 KW that the sort holds are dropped first, by bisection on the high
 // words for one that at least k and at most 32 KW keys reach and, where more than those
-// share the k-th place's high word, on the low ones (their places).
+// share the k-th place's high word, on the low ones (their places).  Entries from `raw`
+// on are not keys yet: their high word is t itself.
 template <int KW>
-__device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
+__device__ __noinline__ int cut(unsigned long long* buf, int raw, int n, int k) {
     constexpr int W = cap_of(KW) / 32;
     const int lane = threadIdx.x & 31;
+    __syncwarp();
+    for (int i = raw + lane; i < n; i += 32)
+        buf[i] = key_of(__uint_as_float((uint32_t)(buf[i] >> 32)), (uint32_t)buf[i]);
     __syncwarp();
     if (n > 32 * KW) {
         // (no key's high word is ~0: that is where float_key puts NaN)
@@ -414,26 +418,42 @@ __device__ __noinline__ int cut(unsigned long long* buf, int n, int k) {
     unsigned long long v[KW];
 #pragma unroll
     for (int r = 0; r < KW; ++r) v[r] = 32 * r + lane < n ? buf[32 * r + lane] : kNone;
+    auto step = [&](int size, int j) {
 #pragma unroll
-    for (int size = 2; size <= 32 * KW; size <<= 1)
+        for (int r = 0; r < KW; ++r) {
+            const unsigned long long p = shfl_xor_u64(v[r], j);
+            const bool up = ((32 * r + lane) & size) == 0, lower = (lane & j) == 0;
+            v[r] = lower == up ? min(v[r], p) : max(v[r], p);
+        }
+    };
+    if constexpr (KW == 1) {
 #pragma unroll
-        for (int j = size >> 1; j > 0; j >>= 1)
+        for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-            for (int r = 0; r < KW; ++r) {
-                if (j >= 32) {
-                    const int o = r ^ (j >> 5);
-                    if (o > r) {
-                        const bool up = ((32 * r) & size) == 0;
-                        const unsigned long long a = min(v[r], v[o]), b = max(v[r], v[o]);
-                        v[r] = up ? a : b;
-                        v[o] = up ? b : a;
-                    }
-                } else {
-                    const unsigned long long p = shfl_xor_u64(v[r], j);
-                    const bool up = ((32 * r + lane) & size) == 0, lower = (lane & j) == 0;
-                    v[r] = lower == up ? min(v[r], p) : max(v[r], p);
-                }
+            for (int j = size >> 1; j > 0; j >>= 1) step(size, j);
+    } else {
+        // rolled: unrolled it is most of the kernel's code, and a fourth of the time of
+        // 4096 rows' best 100 went into fetching that
+        static_assert(KW == 4, "");
+        auto order = [](unsigned long long& a, unsigned long long& b, bool up) {
+            const unsigned long long x = min(a, b), y = max(a, b);
+            a = up ? x : y;
+            b = up ? y : x;
+        };
+#pragma unroll 1
+        for (int size = 2; size <= 128; size <<= 1) {
+            if (size == 128) {
+                order(v[0], v[2], true);
+                order(v[1], v[3], true);
             }
+            if (size >= 64) {
+                order(v[0], v[1], true);
+                order(v[2], v[3], size == 128);
+            }
+#pragma unroll 1
+            for (int j = min(size >> 1, 16); j > 0; j >>= 1) step(size, j);
+        }
+    }
     n = min(n, k);
     __syncwarp();
 #pragma unroll
@@ -541,9 +561,9 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
             edge = load_score(x + edge_at);
         Sums s = no_sums();
         float tau = a.lowest;  // entries below it are not among the best k
-        int n = 0;           // keys in the buffer
+        int n = 0, keys = 0;  // entries in the buffer, and how many of them are keys
         auto sharpen = [&] {
-            n = cut<KW>(sm.buf, n, a.k);
+            n = keys = cut<KW>(sm.buf, keys, n, a.k);
             if (n == a.k) tau = fmaxf(tau, t_of(sm.buf[n - 1]));
         };
         // Appends the lanes' entries (E each) that reach tau.
@@ -556,7 +576,7 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
                 const unsigned ball = __ballot_sync(0xffffffffu, hit);
                 if (hit)
                     sm.buf[n + __popc(ball & ((1u << lane) - 1u))] =
-                        key_of(t[i], (uint32_t)(place + i));
+                        (unsigned long long)__float_as_uint(t[i]) << 32 | (uint32_t)(place + i);
                 n += __popc(ball);
             }
         };
@@ -669,7 +689,7 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
         }
         s = warp_join(s, c);
         int kept = 0;
-        if (a.k > 0) kept = cut<KW>(sm.buf, n, a.k);
+        if (a.k > 0) kept = cut<KW>(sm.buf, keys, n, a.k);
         if (parts == 1) {
             finish_row<T>(a, u.row, u.at, s, sm.buf, kept, c, sgn, lane, 32);
         } else {
@@ -759,7 +779,7 @@ __global__ void __launch_bounds__(128) join_few_parts_kernel(ProbsArgs a, int pa
             n += __popc(ball);
         }
         s = warp_join(s, c);
-        const int kept = a.k > 0 ? cut<KW>(buf, n, a.k) : 0;
+        const int kept = a.k > 0 ? cut<KW>(buf, n, n, a.k) : 0;
         finish_row<T>(a, row, at, s, buf, kept, c, sgn, lane, 32);
         __syncwarp();
     }
