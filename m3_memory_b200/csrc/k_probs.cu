@@ -733,17 +733,42 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(ProbsArgs a, int p
             const float2* v = reinterpret_cast<const float2*>(part_at(a, row * parts + i));
             s = join(s, Sums{v[0].x, v[0].y, v[1].x}, c);
         }
-        int kept = 0;
-        const int total = parts * a.k;
-        for (int b = 0; b < total; b += kTile) {
-            const int n = min(kTile, total - b);
-            for (int i = tid; i < n; i += kThreads) {
-                const int p = (b + i) / a.k, j = (b + i) - p * a.k;
-                sm.buf[kept + i] = reinterpret_cast<const unsigned long long*>(
-                    part_at(a, row * parts + p) + 16)[j];
-            }
+        auto key_at = [&](int p, int j) {
+            return reinterpret_cast<const unsigned long long*>(part_at(a, row * parts + p) +
+                                                               16)[j];
+        };
+        int kept = 0, n = kBuf + 1;
+        if (a.k > 0 && parts >= 2 * a.k) {
+            // many parts: only those whose best key reaches a bound of the k-th best of
+            // all the parts' best ones have any of the row's best k
+            unsigned long long head = kNone;
+            for (int i = tid; i < parts; i += kThreads) head = min(head, key_at(i, 0));
+            if (tid == 0) sm.count = 0;
+            const float b = offered_bound(head == kNone ? ninf() : t_of(head), a.k, sm);
+            const unsigned long long bound = b > ninf() ? key_of(b, 0xFFFFFFFFu) : kNone - 1;
+            for (int i = tid; i < parts; i += kThreads)
+                for (int j = 0; j < a.k; ++j) {
+                    const unsigned long long key = key_at(i, j);
+                    if (key > bound) break;
+                    const int at = atomicAdd(&sm.count, 1);
+                    if (at < kBuf) sm.buf[at] = key;
+                }
             __syncthreads();
-            kept = best_of_buffer(kept + n, a.k, sm);
+            n = sm.count;
+            __syncthreads();
+            if (n <= kBuf) kept = best_of_buffer(n, a.k, sm);
+        }
+        if (n > kBuf) {
+            const int total = parts * a.k;
+            for (int b = 0; b < total; b += kTile) {
+                const int m = min(kTile, total - b);
+                for (int i = tid; i < m; i += kThreads) {
+                    const int p = (b + i) / a.k;
+                    sm.buf[kept + i] = key_at(p, (b + i) - p * a.k);
+                }
+                __syncthreads();
+                kept = best_of_buffer(kept + m, a.k, sm);
+            }
         }
         s = block_join(s, c, sm);
         finish_row<T>(a, row, at, s, sm.buf, kept, c, sgn, tid, kThreads);

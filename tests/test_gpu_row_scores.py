@@ -481,6 +481,15 @@ def test_score_probs_many_equal_scores(R, eng):
         s[2, ::2] = -0.0
         s[2, 1::2] = 0.0
         probs_check(R, eng, s, list(s.float().cpu().numpy()), 3.0, 128)
+    # the best entries all in one part of a long row, and spread one to a part
+    s = randn(1, 600000, seed=5, scale=0.1)
+    s[0, 300000:300200] += 2.0
+    probs_check(R, eng, s, list(s.cpu().numpy()), 4.0, 30)
+    s[0, ::3001] += 3.0
+    for k in (1, 10, 100, 128):
+        probs_check(R, eng, s, list(s.cpu().numpy()), 4.0, k)
+    long = torch.arange(700000, device="cuda", dtype=torch.float32)[None] / 700000
+    probs_check(R, eng, long, list(long.cpu().numpy()), 4.0, 20)
     up = torch.arange(60000, device="cuda", dtype=torch.float32)[None] / 60000
     probs_check(R, eng, up, list(up.cpu().numpy()), 4.0, 128)  # every entry enters the best k
     probs_check(R, eng, -up, list(-up.cpu().numpy()), 4.0, 128)
