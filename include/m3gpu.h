@@ -71,6 +71,8 @@ int m3g_engine_create(m3g_engine** out);
 int m3g_engine_destroy(m3g_engine* e);
 /* Rebind to CUDA device `device` (before any index is created). */
 int m3g_set_device(m3g_engine* e, int device);
+/* The CUDA device the engine is bound to. */
+int m3g_device_of(m3g_engine* e, int* device);
 
 /* AsyncEngine::start / stop (m3_async.cpp:53-105). */
 int m3g_start(m3g_engine* e, int writer_threads, int maintenance_threads);
@@ -347,8 +349,8 @@ int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d
  * streams may overlap, and each may be captured into a CUDA graph (make one call
  * of these before the first capture: it allocates the engine's error word).
  * Enqueued on `stream`; stream NULL: the legacy default stream, waited for.  What
- * a kernel finds wrong on the device (a pair or list out of range, a wait that
- * gave up) is left out and reported by m3g_sync_errors, or by the call itself
+ * a kernel finds wrong on the device (a pair, list or row of scores out of range, a
+ * wait that gave up) is left out and reported by m3g_sync_errors, or by the call itself
  * when it waits.  Inputs and outputs must not overlap.
  *
  * Rows of vectors, one row every `ld` elements:
@@ -358,7 +360,7 @@ int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d
  *             dim i stands for code * 2^(s[i / 128] - 127); s = 255 is not a scale.
  * data starts on a 16-byte boundary and ld is a multiple of 16 bytes; scales
  * starts on a 4-byte boundary and ld_scales is a multiple of 4, at least
- * ceil(dim / 128).  n < 2^31. */
+ * ceil(dim / 128).  n < 2^31, dim <= 2^20. */
 typedef struct {
     const void* data;
     const uint8_t* scales;
@@ -401,7 +403,9 @@ int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, 
 
 /* Scores as probabilities: row i of the scores (dtype M3G_F32 or M3G_BF16) is n
  * entries from element i * ld on, or, with d_row_off [nq + 1] ascending, entries
- * d_row_off[i] .. d_row_off[i + 1] - 1 of n entries in all (ld is not used).  With
+ * d_row_off[i] .. d_row_off[i + 1] - 1 of n entries in all (ld is not used; a row out
+ * of range is taken as one without entries, and reported).  A row holds at most
+ * 2^31 - 2^16 entries.  With
  * l = scale * score (scale finite and not 0), over the entries whose l is neither
  * NaN nor -inf (the others are left out: they have no probability):
  *   out_logsumexp[i] = log sum exp(l)               (-inf where no entry is left)

@@ -64,6 +64,7 @@ SIGNATURES = {
     "m3g_engine_create": (_i32, [ct.POINTER(_vp)]),
     "m3g_engine_destroy": (_i32, [_vp]),
     "m3g_set_device": (_i32, [_vp, _i32]),
+    "m3g_device_of": (_i32, [_vp, _pi]),
     "m3g_start": (_i32, [_vp, _i32, _i32]),
     "m3g_stop": (_i32, [_vp]),
     "m3g_set_queue_policy": (_i32, [_vp, _sz, _sz, _i32]),
@@ -191,6 +192,7 @@ class Engine:
         h = ct.c_void_p()
         check(lib().m3g_engine_create(ct.byref(h)))
         self.h = h
+        self._dev = None  # device(), once asked for
 
     def close(self):
         if getattr(self, "h", None):
@@ -204,6 +206,19 @@ class Engine:
             self.close()
         except TypeError:
             pass
+
+    def device(self):
+        """The index of the CUDA device the engine is bound to."""
+        if self._dev is None:
+            d = ct.c_int()
+            check(lib().m3g_device_of(self.h, ct.byref(d)))
+            self._dev = d.value
+        return self._dev
+
+    def set_device(self, device):
+        """Rebinds to another CUDA device, before the engine is used."""
+        check(lib().m3g_set_device(self.h, device))
+        self._dev = None
 
     # lifecycle / policies
     def start(self, writers=2, maint=1):

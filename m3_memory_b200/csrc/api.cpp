@@ -571,6 +571,14 @@ int m3g_score_probs_device(m3g_engine* e, const void* d_scores, int dtype, int64
     });
 }
 
+int m3g_device_of(m3g_engine* e, int* device) {
+    M3G_ENGINE_OR_FAIL(e);
+    return guarded([&] {
+        if (!device) m3g::fail(M3G_EINVAL, "device_of: out missing");
+        *device = e->eng.device();
+    });
+}
+
 int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d_centroids,
                               int64_t nlist, int dim, int metric, int normalized, int nprobe,
                               int32_t* d_out_probes, void* stream) {

@@ -274,9 +274,10 @@ struct RowAt {
 };
 __device__ __forceinline__ RowAt row_at(const ProbsArgs& a, int64_t row) {
     if (!a.row_off) return {row * a.ld, a.n};
-    const int64_t b = max((int64_t)0, min(a.row_off[row], a.n));
-    const int64_t len = max((int64_t)0, min(a.row_off[row + 1], a.n) - b);
-    return {b, min(len, (int64_t)INT32_MAX)};
+    const int64_t b = a.row_off[row], e = a.row_off[row + 1];
+    if (b >= 0 && b <= e && e <= a.n && e - b <= kProbsMaxRow) return {b, e - b};
+    atomicOr(a.err + kScoreBadItem, 1);
+    return {0, 0};
 }
 
 // l = c t, or the reference value where that is infinite
@@ -491,7 +492,7 @@ struct Unit {
 
 template <class T, int KW>
 __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
-    score_probs_kernel(ProbsArgs a, int parts, int* err) {
+    score_probs_kernel(ProbsArgs a, int parts) {
     constexpr int V = Vec<T>::kN;
     extern __shared__ unsigned char smem_raw[];
     const int lane = threadIdx.x & 31;
@@ -706,7 +707,7 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
     if (lost) {
         // no copy may still be landing when the warp leaves
         if (lane == 0) {
-            atomicOr(err + kScoreTimeout, 1);
+            atomicOr(a.err + kScoreTimeout, 1);
             for (uint32_t k = used; k != issued; ++k)
                 mbar_drain(&sm.full[k % kStages], (k / kStages) & 1u);
         }
@@ -835,7 +836,7 @@ cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, 
 }
 
 template <class T, int KW>
-cudaError_t launch_kw(const ProbsArgs& a, int parts, int* err, int sms, cudaStream_t st) {
+cudaError_t launch_kw(const ProbsArgs& a, int parts, int sms, cudaStream_t st) {
     constexpr int smem = (int)sizeof(WarpShared<KW>) * warps_of(KW) + 128;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     static std::atomic<uint64_t> set{0};  // a bit a device
@@ -850,7 +851,7 @@ cudaError_t launch_kw(const ProbsArgs& a, int parts, int* err, int sms, cudaStre
         set |= bit;
     }
     const unsigned grid = (unsigned)std::min<int64_t>(a.nq * parts, sms);
-    score_probs_kernel<T, KW><<<grid, warps_of(KW) * 32, smem, st>>>(a, parts, err);
+    score_probs_kernel<T, KW><<<grid, warps_of(KW) * 32, smem, st>>>(a, parts);
     e = cudaGetLastError();
     if (e != cudaSuccess || parts == 1) return e;
     if ((int64_t)parts * a.k <= cap_of(KW) && parts <= 256)
@@ -868,13 +869,13 @@ int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, i
     return parts == 1 ? 0 : nq * parts * (16 + 8 * (int64_t)k);
 }
 
-cudaError_t launch_score_probs(const ProbsArgs& a, int* err, int sms, cudaStream_t st) {
+cudaError_t launch_score_probs(const ProbsArgs& a, int sms, cudaStream_t st) {
     const int parts = parts_of(a.nq, a.n, a.row_off != nullptr, element_size(a.dtype), sms);
     if (a.dtype == M3G_F32)
-        return a.k <= 32 ? launch_kw<float, 1>(a, parts, err, sms, st)
-                         : launch_kw<float, 4>(a, parts, err, sms, st);
-    return a.k <= 32 ? launch_kw<__nv_bfloat16, 1>(a, parts, err, sms, st)
-                     : launch_kw<__nv_bfloat16, 4>(a, parts, err, sms, st);
+        return a.k <= 32 ? launch_kw<float, 1>(a, parts, sms, st)
+                         : launch_kw<float, 4>(a, parts, sms, st);
+    return a.k <= 32 ? launch_kw<__nv_bfloat16, 1>(a, parts, sms, st)
+                     : launch_kw<__nv_bfloat16, 4>(a, parts, sms, st);
 }
 
 }  // namespace m3g

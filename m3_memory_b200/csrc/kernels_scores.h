@@ -34,7 +34,9 @@ cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const Score
                                float alpha, float beta, void* out, int out_dtype, int* err,
                                int sms, cudaStream_t st);
 
+constexpr int kScoreMaxDim = 1 << 20;        // dims of a row
 constexpr int kProbsMaxK = 128;
+constexpr int64_t kProbsMaxRow = 0x7FFF0000;  // entries of a row: places in it are ints
 int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, int sms);
 struct ProbsArgs {
     const void* scores;
@@ -49,7 +51,8 @@ struct ProbsArgs {
     int64_t* top_index;
     float* top;
     void* work;
+    int* err;
 };
-cudaError_t launch_score_probs(const ProbsArgs& a, int* err, int sms, cudaStream_t st);
+cudaError_t launch_score_probs(const ProbsArgs& a, int sms, cudaStream_t st);
 
 }  // namespace m3g

@@ -21,6 +21,7 @@ void check_rows(const char* who, const char* name, const m3g_rows* r) {
         fail(M3G_EINVAL, at + "rows are bf16 or e4m3");
     if (r->n < 0 || r->dim <= 0) fail(M3G_EINVAL, at + "bad sizes");
     if (r->n > INT32_MAX) fail(M3G_EUNSUPPORTED, at + "2^31 rows or more");
+    if (r->dim > kScoreMaxDim) fail(M3G_EUNSUPPORTED, at + "more than 2^20 dims");
     const int64_t esize = r->dtype == M3G_BF16 ? 2 : 1;
     if (r->ld < r->dim || r->ld > kMaxLd || (r->ld * esize) % 16 != 0)
         fail(M3G_EINVAL, at + "ld must be at least dim and a multiple of 16 bytes");
@@ -87,7 +88,7 @@ void Engine::row_score_errors() {
         M3G_CK(cudaMemset(score_err_.p, 0, sizeof(w)));
     if (w[kScoreTimeout]) fail(M3G_ETIMEOUT, "row scores: a device-side wait gave up");
     if (w[kScoreBadItem])
-        fail(M3G_ERANGE, "row scores: a list or pair out of range was left out");
+        fail(M3G_ERANGE, "row scores: a list, pair or row of scores out of range was left out");
 }
 
 void Engine::pack_rows(const void* dX, int dtype, int64_t n, int dim, int64_t ldx,
@@ -156,8 +157,8 @@ void Engine::score_probs(ProbsArgs a, int64_t work_bytes, cudaStream_t ext) {
     if (a.k > kProbsMaxK)
         fail(M3G_EUNSUPPORTED,
              "score_probs: k > " + std::to_string(kProbsMaxK) + " is not supported");
-    if (a.nq > INT32_MAX || (!a.row_off && a.n > INT32_MAX) || a.n > kMaxLd)
-        fail(M3G_EUNSUPPORTED, "score_probs: 2^31 rows or entries in a row, or more");
+    if (a.nq > INT32_MAX || (!a.row_off && a.n > kProbsMaxRow) || a.n > kMaxLd)
+        fail(M3G_EUNSUPPORTED, "score_probs: 2^31 - 2^16 entries in a row, or 2^31 rows");
     if (!a.row_off && (a.ld < a.n || a.ld > kMaxLd))
         fail(M3G_EINVAL, "score_probs: ld must be at least n");
     if (!std::isfinite(a.scale) || a.scale == 0.f)
@@ -176,7 +177,8 @@ void Engine::score_probs(ProbsArgs a, int64_t work_bytes, cudaStream_t ext) {
                              " bytes on an 8-byte boundary");
     DeviceGuard g(device_);
     a.lowest = lowest_score(std::fabs(a.scale));
-    M3G_CK(launch_score_probs(a, score_err(), num_sms_, ext));
+    a.err = score_err();
+    M3G_CK(launch_score_probs(a, num_sms_, ext));
     if (!ext) row_score_errors();
 }
 

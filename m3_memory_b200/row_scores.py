@@ -69,10 +69,13 @@ def _bad(what, msg):
     raise ValueError(f"{what} {msg}")
 
 
-def _device_of(t, what):
+def _device_of(engine, t, what):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _bad(what, "must be a CUDA tensor")
-    return t.get_device()
+    dev = t.get_device()
+    if dev != engine.device():
+        _bad(what, f"is on {t.device}, the engine on cuda:{engine.device()}")
+    return dev
 
 
 def _vector(t, dtype, n, dev, what):
@@ -130,14 +133,14 @@ def _dtype(t, what):
     return d
 
 
-def _device(rows, what):
-    return _device_of(rows.codes if isinstance(rows, PackedRows) else rows, what)
+def _device(engine, rows, what):
+    return _device_of(engine, rows.codes if isinstance(rows, PackedRows) else rows, what)
 
 
 def pack_rows(engine, x, out=None) -> PackedRows:
     """Packs fp32 or bf16 rows ``x [n, dim]`` to 8 bits (m3g_pack_rows_device): e4m3 codes with one
     power-of-two scale per 128 dims.  ``out``: PackedRows to write instead of new ones."""
-    dev = _device_of(x, "x")
+    dev = _device_of(engine, x, "x")
     dtype = _dtype(x.dtype, "x")
     n, dim, ldx = _matrix(x, dev, "x")
     if out is None:
@@ -156,7 +159,7 @@ def pack_rows(engine, x, out=None) -> PackedRows:
 def row_scores(engine, q, x, alpha=1.0, beta=0.0, out_dtype=torch.float32, out=None):
     """``alpha * q @ x.T + beta`` for every row of q and x (m3g_row_scores_device), ``[len(q),
     len(x)]`` in float32 or bfloat16.  ``out``: a matrix to write instead of a new one."""
-    dev = _device(x, "x")
+    dev = _device(engine, x, "x")
     a, b = _rows(q, dev, "q"), _rows(x, dev, "x")
     if out is None:
         _dtype(out_dtype, "out_dtype")
@@ -181,7 +184,7 @@ def list_scores(engine, q, x, list_off, list_len, pair_off, out_off, out, pair_r
     ``pair_off[g] .. pair_off[g + 1]`` (int64, one entry more) probe it; pair p is row
     ``pair_row[p]`` of q (int32; row p without it, -1 for none) and writes ``list_len[g]`` scores
     from ``out[out_off[p]]`` (int64) on."""
-    dev = _device(x, "x")
+    dev = _device(engine, x, "x")
     a, b = _rows(q, dev, "q"), _rows(x, dev, "x")
     ngroup, npair, n = list_off.numel(), out_off.numel(), out.numel()
     engine.list_scores_device(
@@ -200,7 +203,7 @@ def score_probs(engine, scores, scale=1.0, k=0, given=None, row_off=None) -> Sco
     places in the row; -1 for none) and the k most probable entries.  Entries that are NaN, or
     -inf after scaling, are left out.  ``scores``: float32 or bfloat16 ``[nq, n]``, or a vector
     whose row i is ``scores[row_off[i]:row_off[i + 1]]`` (``row_off`` int64)."""
-    dev = _device_of(scores, "scores")
+    dev = _device_of(engine, scores, "scores")
     dtype = _dtype(scores.dtype, "scores")
     off = None
     if row_off is None:

@@ -508,6 +508,23 @@ def test_score_probs_extremes(R, eng):
     assert got.top_index.item() == 1
 
 
+def test_score_probs_bad_rows_reported(R, eng):
+    """Row offsets that fall, or leave the scores: those rows count as empty, the others are right."""
+    s = some_scores(1, 1000, torch.float32, 2)[0]
+    f = s.cpu().numpy()
+    off = [0, 100, 90, 300, 2000, 400, 500, -5, 10]
+    good = [(a, b) if 0 <= a <= b <= 1000 else (0, 0) for a, b in zip(off, off[1:])]
+    t = torch.tensor(off, device="cuda")
+    got = R.score_probs(eng, s, scale=3.0, k=4, row_off=t)
+    with pytest.raises(IndexError):
+        eng.sync_errors()
+    eng.sync_errors()
+    for i, (a, b) in enumerate(good):
+        r = probs_ref([f[a:b]], 3.0, 4, None)[0]
+        assert close(got.logsumexp[i].item(), r[0], r[5])
+        assert np.array_equal(got.top_index[i].cpu().numpy(), r[4])
+
+
 def test_score_probs_no_rows_or_entries(R, eng):
     got = R.score_probs(eng, torch.empty(0, 5, device="cuda"), k=2)
     assert got.top.shape == (0, 2)
@@ -668,6 +685,26 @@ def test_two_graphs_of_one_retrieval(R, eng):
             assert torch.equal(p.entropy, outs[i][1].entropy)
     eng.sync_errors()
     del graphs
+
+
+def test_graph_of_split_rows(R, eng):
+    """Rows split over blocks (two kernels) captured and replayed with new scores, eager calls of
+    the same shape between."""
+    s = some_scores(3, 60001, torch.float32, 1)
+    R.score_probs(eng, s, scale=4.0, k=6)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = R.score_probs(eng, s, scale=4.0, k=6)
+    for rep in range(4):
+        new = some_scores(3, 60001, torch.float32, 10 + rep)
+        s.copy_(new)
+        g.replay()
+        want = R.score_probs(eng, new, scale=4.0, k=6)
+        torch.cuda.synchronize()
+        assert torch.equal(got.logsumexp, want.logsumexp)
+        assert torch.equal(got.top_index, want.top_index) and torch.equal(got.top, want.top)
+    del g
 
 
 def test_null_stream_waits_and_reports(R, eng):

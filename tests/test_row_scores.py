@@ -40,9 +40,11 @@ def test_rows_refused(eng, bad, side):
         eng.list_scores_device(q, x, 1, P, P, P, 1, P, P, 1.0, 0.0, P, cabi.F32, 8)
 
 
-def test_too_many_rows_unsupported(eng):
+@pytest.mark.parametrize("big", [dict(n=1 << 31), dict(dim=(1 << 20) + 1, ld=1 << 21,
+                                                       ld_scales=1 << 16)])
+def test_too_many_rows_or_dims_unsupported(eng, big):
     with pytest.raises(cabi.M3GError) as ei:
-        eng.row_scores_device(rows(), rows(n=1 << 31), 1.0, 0.0, P, cabi.F32, 1 << 31)
+        eng.row_scores_device(rows(), rows(**big), 1.0, 0.0, P, cabi.F32, 1 << 31)
     assert ei.value.code == UNSUPPORTED
 
 
@@ -135,6 +137,12 @@ def test_empty_calls_touch_nothing(eng):
                            cabi.F32, 0)
     eng.score_probs_device(None, cabi.F32, 0, 0, 0, None, 1.0, None, 0, 0, None, None, None, None,
                            None, None, 0)
+
+
+def test_device_of(eng):
+    assert eng.device() == 0
+    assert cabi.lib().m3g_device_of(eng.h, None) == cabi.M3G_EINVAL
+    assert cabi.lib().m3g_device_of(None, None) == cabi.M3G_EINVAL
 
 
 def test_storage_stays_fp32_or_bf16(eng):
