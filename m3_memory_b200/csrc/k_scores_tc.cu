@@ -27,16 +27,11 @@
 #include <type_traits>
 
 #include "common.cuh"
-#include "kernels.h"
-#include "kernels_scores.h"
-#include "tc.cuh"
+#include "scores_tc.cuh"
 
 namespace m3g {
 namespace {
 
-constexpr int kM = 128;                 // rows of x a tile
-constexpr int kSlice = 128;             // bytes of a row a swizzled tile holds (128 8-bit or 64 bf16 dims)
-constexpr int kXBytes = kM * kSlice;
 constexpr int kEpiWarps = 8;            // two for each quarter of the TMEM lanes
 constexpr int kQueryWarps = 4;          // each gathers every fourth stage's queries
 constexpr int kScaleWarps = 4;          // one for each quarter of the TMEM lanes
@@ -125,41 +120,6 @@ __device__ __forceinline__ void tc_mma_mx(uint32_t d, uint64_t a, uint64_t b, ui
         "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)accumulate)
         : "memory");
 }
-
-// One word a lane into each of four TMEM columns of the warp's lane quarter.
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c,
-                                         uint32_t d) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
-                 "r"(a), "r"(b), "r"(c), "r"(d)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// kind::mxf8f6f4: both operands e4m3 (0) and K-major, N >> 3 at bits 17-22, ue8m0
-// scales (bit 23), M >> 7 at bits 27-28; the scale byte of the words: bits 4-5 (B)
-// and 29-30 (A).
-__device__ __forceinline__ uint32_t mx_idesc(int n) {
-    return ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27);
-}
-__device__ __forceinline__ uint32_t mx_idesc_byte(uint32_t idesc, int byte) {
-    return idesc | ((uint32_t)byte << 4) | ((uint32_t)byte << 29);
-}
-
-// A position in a ring of N slots and the parity of its current round.
-template <int N>
-struct Ring {
-    __device__ static constexpr uint32_t slots() { return N; }
-    uint32_t i = 0, phase = 0, n = 0;
-    __device__ __forceinline__ void next() {
-        ++n;
-        if (++i == N) {
-            i = 0;
-            phase ^= 1u;
-        }
-    }
-};
 
 // A group's tiles: its rows in 128s (nx) times its pairs in nqt parts of `per`, the
 // pairs fastest.  CTAs take runs of equal weight: a tile of 32 b rows weighs 1 + 2 b
@@ -439,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             tc_fence_after();
             const uint32_t d = tmem + (uint32_t)(h * S::kAcc);
-            const uint32_t idesc = F8 ? mx_idesc(n) : tc_idesc_m128(n, 1);
+            const uint32_t idesc = F8 ? mx_idesc(kM, n) : tc_idesc_m128(n, 1);
             for (int kt = 0; kt < p.nk; kt += S::kSlices) {
                 const bool first = F8 && (kt & 3) == 0;
                 const bool end = kt + S::kSlices >= p.nk;
@@ -714,14 +674,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-void row_map(CUtensorMap* m, const m3g_rows& r, int box_rows) {
-    const bool f8 = r.dtype == M3G_E4M3;
-    encode_tma_2d(m, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r.data,
-                  (uint64_t)r.dim, (uint64_t)r.n, (uint64_t)r.ld * (f8 ? 1 : 2),
-                  (uint32_t)(f8 ? kSlice : kSlice / 2), (uint32_t)box_rows,
-                  CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <bool F8, int NT, bool GROUP, class O>
 cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* out,
                    unsigned grid, cudaStream_t st) {
@@ -761,7 +713,8 @@ cudaError_t launch_any(const m3g_rows& q, const m3g_rows& x, const Params& p, in
     };
     if (queries <= 32) return with(std::integral_constant<int, 32>());
     if (queries <= 64) return with(std::integral_constant<int, 64>());
-    return with(std::integral_constant<int, 240>());
+    if constexpr (GROUP) return with(std::integral_constant<int, 240>());
+    else return cudaErrorInvalidValue;  // (launch_pair_scores)
 }
 
 Params params_of(const m3g_rows& q, const m3g_rows& x, float alpha, float beta, int* err) {
@@ -787,6 +740,7 @@ Params params_of(const m3g_rows& q, const m3g_rows& x, float alpha, float beta, 
 cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
                               void* out, int out_dtype, int64_t ld_out, int* err, int sms,
                               cudaStream_t st) {
+    if (q.n > 64) return launch_pair_scores(q, x, alpha, beta, out, out_dtype, ld_out, err, sms, st);
     Params p = params_of(q, x, alpha, beta, err);
     p.ld_out = ld_out;
     const int64_t tiles = (x.n + kM - 1) / kM * ((q.n + 15) / 16);  // at least as many as there are
