@@ -374,28 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             tc_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(h * kAcc);
             if (quarter * 32 < r.nx) {
-                O* mine = out + (int64_t)r.q0 * p.ld_out + r.x0 + row;
-                const bool in = row < r.nx;
-#pragma unroll 1
-                for (int c0 = 16 * half; c0 < r.nq; c0 += 32) {
-                    uint32_t v[16];
-                    tmem_ld16(acc + (uint32_t)c0, v);
-                    auto put = [&](int u) {
-                        const float s = fmaf(p.alpha, __uint_as_float(v[u]), p.beta);
-                        if (in) {
-                            if constexpr (sizeof(O) == 4) mine[(c0 + u) * p.ld_out] = s;
-                            else mine[(c0 + u) * p.ld_out] = __float2bfloat16_rn(s);
-                        }
-                    };
-                    if (c0 + 16 <= r.nq) {
-#pragma unroll
-                        for (int u = 0; u < 16; ++u) put(u);
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 16; ++u)
-                            if (c0 + u < r.nq) put(u);
-                    }
-                }
+                store_columns(out + (int64_t)r.q0 * p.ld_out + r.x0 + row, p.ld_out, acc, half,
+                              r.nq, row < r.nx, p.alpha, p.beta);
             }
             tc_fence_before();
             __syncwarp();

@@ -49,6 +49,65 @@ struct Ring {
     }
 };
 
+__device__ __forceinline__ void put_score(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put_score(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// 16 columns of the warp's TMEM lanes, waited for by tmem_ld_wait.
+__device__ __forceinline__ void tmem_ld16_start(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// The values of r are there after it (and not read before it).
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+// Every other 16 of a tile's nq columns, from 16 * half on: a lane stores its row's
+// score of column c at mine[c * ld].  The next columns are on their way from TMEM while
+// these are stored (a load waited for at once, and a multiplication for each address,
+// cost 690 cycles for 16 columns where the stores take 400).
+template <class O>
+__device__ __forceinline__ void store_columns(O* mine, int64_t ld, uint32_t acc, int half, int nq,
+                                              bool in, float alpha, float beta) {
+    uint32_t cur[16], next[16];
+    int c = 16 * half;
+    if (c >= nq) return;
+    O* at = mine + c * ld;
+    tmem_ld16_start(acc + (uint32_t)c, cur);
+#pragma unroll 1
+    for (; c < nq; c += 32) {
+        tmem_ld_wait(cur);
+        if (c + 32 < nq) tmem_ld16_start(acc + (uint32_t)(c + 32), next);
+        if (c + 16 <= nq) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                if (in) put_score(at, fmaf(alpha, __uint_as_float(cur[u]), beta));
+                at += ld;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                if (in && c + u < nq) put_score(at, fmaf(alpha, __uint_as_float(cur[u]), beta));
+                at += ld;
+            }
+        }
+        at += 16 * ld;
+        tmem_ld_wait(next);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) cur[u] = next[u];
+    }
+}
+
 // The map of rows in boxes of a slice and box_rows rows, 128-byte swizzle.
 inline void row_map(CUtensorMap* m, const m3g_rows& r, int box_rows) {
     const bool f8 = r.dtype == M3G_E4M3;
