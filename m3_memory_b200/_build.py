@@ -26,11 +26,10 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
               *ARCH, f"-I{INCLUDE}", f"-I{CSRC}"]
 
 CU_SOURCES = ["k_coarse.cu", "k_scan.cu", "k_scan_tc.cu", "k_kmeans.cu", "k_gemm_tc.cu",
-              "engine.cu", "noalloc.cu", "k_pack.cu", "k_scores_tc.cu",
-              "k_scores_pair.cu", "k_probs.cu"]
+              "engine.cu", "noalloc.cu", "k_pack.cu", "k_scores_tc.cu", "k_probs.cu"]
 CPP_SOURCES = ["api.cpp", "faiss_io.cpp", "row_scores.cpp"]
 HEADERS = ["common.cuh", "score.cuh", "topk.cuh", "tc.cuh", "kernels.h", "kernels_kmeans.h",
-           "kernels_scores.h", "scores_tc.cuh", "engine.h"]
+           "kernels_scores.h", "engine.h"]
 
 
 def _newer(target: Path, deps) -> bool:

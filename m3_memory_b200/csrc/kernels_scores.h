@@ -1,5 +1,5 @@
 // kernels_scores.h -- launchers of the row-score kernels (k_pack.cu, k_scores_tc.cu,
-// k_scores_pair.cu, k_probs.cu).
+// k_probs.cu).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -30,10 +30,6 @@ cudaError_t launch_pack_rows(const void* x, int dtype, int64_t n, int dim, int64
 cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
                               void* out, int out_dtype, int64_t ld_out, int* err, int sms,
                               cudaStream_t st);
-// The dense form with more than 64 queries (k_scores_pair.cu).
-cudaError_t launch_pair_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
-                               void* out, int out_dtype, int64_t ld_out, int* err, int sms,
-                               cudaStream_t st);
 cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const ScoreGroups& g,
                                float alpha, float beta, void* out, int out_dtype, int* err,
                                int sms, cudaStream_t st);
