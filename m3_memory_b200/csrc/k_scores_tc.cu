@@ -318,21 +318,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&map_q);
     }
 
-    // This CTA's tiles.  Grouped: a run of the launch's weight, which is added up first,
-    // each thread a run of groups.  Dense: every gridDim.x-th tile.
+    // This CTA's tiles.  Grouped: a run of the launch's weight, which is added up first:
+    // runs of `chunk` groups by warps, then over the runs by threads.  Dense: every
+    // gridDim.x-th tile.
     int64_t total;
-    int64_t chunk = 0;  // groups a thread counts
+    int64_t chunk = 0;  // groups of a run (a multiple of 32)
     if constexpr (GROUP) {
-        chunk = (p.g.ngroup + kThreads - 1) / kThreads;
-        const int64_t g0 = chunk * threadIdx.x, g1 = min(g0 + chunk, p.g.ngroup);
-        int64_t mine = 0;
+        chunk = 32 * ((p.g.ngroup + 32 * kThreads - 1) / (32 * (int64_t)kThreads));
+        sm.prefix[threadIdx.x] = 0;
+        __syncthreads();
         bool ok = true;
 #pragma unroll 4
-        for (int64_t i = g0; i < g1; ++i) {
-            GroupAt at;
-            ok &= load_group(p, i, &at);
-            mine += Tiles<NT>(at.len, at.m).weight();
+        for (int64_t b = warp; b < kThreads; b += kThreads / 32) {
+            if (b * chunk >= p.g.ngroup) break;
+            int64_t sum = 0;
+            for (int64_t i = b * chunk + lane; i < min((b + 1) * chunk, p.g.ngroup); i += 32) {
+                GroupAt at;
+                ok &= load_group(p, i, &at);
+                sum += Tiles<NT>(at.len, at.m).weight();
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) sm.prefix[b] = sum;
         }
+        __syncthreads();
+        const int64_t mine = sm.prefix[threadIdx.x];
         if (!ok && blockIdx.x == 0) atomicOr(p.err + kScoreBadItem, 1);
         int64_t incl = mine;
 #pragma unroll
