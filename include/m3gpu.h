@@ -394,7 +394,7 @@ int m3g_row_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, f
  * d_out_off[p] on (elements no pair writes keep their values; pairs must not
  * share elements).  d_pair_off [ngroup + 1] ascending from 0 to npair.  out_n:
  * the elements of d_out; pairs whose scores would end past it are left out and
- * reported, as are lists and pairs out of range. */
+ * reported, as are lists and pairs out of range.  ngroup <= 2^22, npair < 2^31. */
 int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, int64_t ngroup,
                            const int64_t* d_list_off, const int32_t* d_list_len,
                            const int64_t* d_pair_off, int64_t npair, const int32_t* d_pair_row,

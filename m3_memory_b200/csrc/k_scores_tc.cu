@@ -16,9 +16,24 @@
 // kind::f16.  Sums are fp32 in TMEM.
 //
 // A launch is one CTA per SM.  A tile is 128 rows of a group and up to NT of its
-// queries, queries fastest, so the rows come from L2 after their first tile.  Warp 0 loads rows and warp 12 queries (TMA; those of a group
-// are gathered by warps 12-15), warp 1 issues the MMAs, warp 3 walks the groups and
-// queues tiles, warps 4-11 store, warps 16-19 bring scale words.  Every wait is bounded.
+// queries, queries fastest, so the rows come from L2 after their first tile.  Warp 0
+// loads rows and warp 12 queries (TMA; those of a group are gathered by warps 12-15),
+// warp 1 issues the MMAs, warp 3 walks the groups and queues tiles, warps 4-11 store,
+// warps 16-19 bring scale words.  Every wait is bounded.
+//
+// What bounds it, and what it measured:
+//   few queries a row: the rows' bytes.  One query against 1M x 1024 8-bit rows 157 us
+//     (6.6 TB/s); 1024 queries x 32 of 4096 lists, 1M x 1024 8-bit rows 194 us (5.3);
+//     4096 x 16 of 4096 lists, 1M x 768 bf16 rows 257 us (5.9; partly filled tiles cost
+//     the MMA warp as much as full ones, and a tile of 8-bit rows has fewer bytes).
+//   many queries: the operands through L2, 46 KB for 128 bytes of K of a 128 x 240 tile
+//     at the 40 bytes a cycle L2 gives an SM, and the scores' own bytes.  1024 queries x
+//     100096 rows x 1024 dims 142 us (1480 TFLOP/s), 4096 x 16384 x 768 bf16 94 us
+//     (1100).  Rows of scores that do not start on 32-byte boundaries cost up to 1.8
+//     times their bytes: every 32-row store ends inside sectors (x 128 dims: 87 us where
+//     n is a multiple of 8, 150 where it is odd).  CTA pairs (cta_group::2, 31 KB of
+//     operands a CTA) took 150 and 88 us, staging the scores through shared memory for
+//     16-byte stores 164: neither was kept.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -106,7 +121,9 @@ struct Params {
     int* err;
 };
 
-// 16 bytes global -> shared, those past the first `size` filled with zeros.
+// 16 bytes global -> shared, those past the first `size` filled with zeros.  Through
+// L1: a list's next tile gathers the same rows (215 us for 195 without, 1024 x 32 of
+// 4096 lists).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size)
                  : "memory");

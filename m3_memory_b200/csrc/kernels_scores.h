@@ -35,6 +35,7 @@ cudaError_t launch_list_scores(const m3g_rows& q, const m3g_rows& x, const Score
                                int sms, cudaStream_t st);
 
 constexpr int kScoreMaxDim = 1 << 20;        // dims of a row
+constexpr int64_t kScoreMaxGroups = 1 << 22; // lists of a call: one warp may walk them all
 constexpr int kProbsMaxK = 128;
 constexpr int64_t kProbsMaxRow = 0x7FFF0000;  // entries of a row: places in it are ints
 int64_t score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k, int sms);

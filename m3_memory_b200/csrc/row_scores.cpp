@@ -127,8 +127,8 @@ void Engine::list_scores(const m3g_rows* q, const m3g_rows* x, const ScoreGroups
     check_pair("list_scores", q, x, out_dtype, alpha, beta);
     const ScoreGroups& s = groups;
     if (s.ngroup < 0 || s.npair < 0 || s.out_n < 0) fail(M3G_EINVAL, "list_scores: bad sizes");
-    if (s.ngroup > INT32_MAX || s.npair > INT32_MAX)
-        fail(M3G_EUNSUPPORTED, "list_scores: 2^31 lists or pairs, or more");
+    if (s.ngroup > kScoreMaxGroups || s.npair > INT32_MAX)
+        fail(M3G_EUNSUPPORTED, "list_scores: more than 2^22 lists, or 2^31 pairs");
     if (s.ngroup == 0 || s.npair == 0 || q->n == 0 || x->n == 0 || s.out_n == 0) return;
     if (!s.list_off || !s.list_len || !s.pair_off || !s.out_off)
         fail(M3G_EINVAL, "list_scores: buffers missing");

@@ -84,7 +84,7 @@ def test_list_scores_refused(eng, case):
 
 
 def test_list_scores_sizes_unsupported(eng):
-    for ngroup, npair in ((1 << 31, 3), (2, 1 << 31)):
+    for ngroup, npair in (((1 << 22) + 1, 3), (2, 1 << 31)):
         with pytest.raises(cabi.M3GError) as ei:
             eng.list_scores_device(rows(), rows(), ngroup, P, P, P, npair, P, P, 1.0, 0.0, P,
                                    cabi.F32, 64)
