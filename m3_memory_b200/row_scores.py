@@ -65,6 +65,15 @@ def _stream(dev):
     return _raw_stream(dev) or _LEGACY_STREAM
 
 
+def _matrix_of(n, d, dtype, device):
+    """A new contiguous matrix (the cheapest way to one)."""
+    return torch.empty_strided((n, d), (d or 1, 1), dtype=dtype, device=device)
+
+
+def _vector_of(n, dtype, device):
+    return torch.empty_strided((n,), (1,), dtype=dtype, device=device)
+
+
 def _bad(what, msg):
     raise ValueError(f"{what} {msg}")
 
@@ -147,8 +156,8 @@ def pack_rows(engine, x, out=None) -> PackedRows:
         if dim == 0:
             _bad("x", "has no dims")
         nblk = (dim + BLOCK - 1) // BLOCK
-        out = PackedRows(x.new_empty((n, (dim + 15) // 16 * 16), dtype=_U8),
-                         x.new_empty((n, (nblk + 3) // 4 * 4), dtype=_U8), dim)
+        out = PackedRows(_matrix_of(n, (dim + 15) // 16 * 16, _U8, x.device),
+                         _matrix_of(n, (nblk + 3) // 4 * 4, _U8, x.device), dim)
     elif out.dim != dim or out.codes.shape[0] != n:
         _bad("out", f"does not hold {n} rows of {dim} dims")
     engine.pack_rows_device(x.data_ptr(), dtype, n, dim, ldx, _rows(out, dev, "out"),
@@ -164,7 +173,7 @@ def row_scores(engine, q, x, alpha=1.0, beta=0.0, out_dtype=torch.float32, out=N
     if out is None:
         _dtype(out_dtype, "out_dtype")
         t = x.codes if isinstance(x, PackedRows) else x
-        out = t.new_empty((a.n, b.n), dtype=out_dtype)
+        out = _matrix_of(a.n, b.n, out_dtype, t.device)
         ld = b.n
     else:
         n, d, ld = _matrix(out, dev, "out")
@@ -215,7 +224,7 @@ def score_probs(engine, scores, scale=1.0, k=0, given=None, row_off=None) -> Sco
             _bad("row_off", "holds one entry more than there are rows")
         _vector(scores, scores.dtype, n, dev, "scores")
         off = _vector(row_off, _I64, nq + 1, dev, "row_off")
-    ngiven, given_at = 0, None
+    on, ngiven, given_at = scores.device, 0, None
     out_given = top = top_index = work = None
     if given is not None:
         if given.dtype != _I64 or not given.is_contiguous():
@@ -223,15 +232,14 @@ def score_probs(engine, scores, scale=1.0, k=0, given=None, row_off=None) -> Sco
         g, ngiven, _ = _matrix(given, dev, "given")
         if g != nq:
             _bad("given", f"must have {nq} rows")
-        out_given = scores.new_empty((nq, ngiven), dtype=_F32)
+        out_given = _matrix_of(nq, ngiven, _F32, on)
         given_at = given.data_ptr() if ngiven else None
-    lse, entropy = scores.new_empty((2, nq), dtype=_F32).unbind()
+    lse, entropy = _vector_of(nq, _F32, on), _vector_of(nq, _F32, on)
     if k > 0:
-        top = scores.new_empty((nq, k), dtype=_F32)
-        top_index = scores.new_empty((nq, k), dtype=_I64)
+        top, top_index = _matrix_of(nq, k, _F32, on), _matrix_of(nq, k, _I64, on)
     nbytes = engine.score_probs_work(nq, n, off is not None, dtype, k)
     if nbytes:
-        work = scores.new_empty(nbytes, dtype=_U8)
+        work = _vector_of(nbytes, _U8, on)
     engine.score_probs_device(
         scores.data_ptr(), dtype, nq, n, ld, off, scale, given_at, ngiven, k, lse.data_ptr(),
         entropy.data_ptr(), out_given.data_ptr() if ngiven else None,
