@@ -23,7 +23,7 @@
 //
 // What bounds it, and what it measured:
 //   few queries a row: the rows' bytes.  One query against 1M x 1024 8-bit rows 157 us
-//     (6.6 TB/s); 1024 queries x 32 of 4096 lists, 1M x 1024 8-bit rows 194 us (5.3);
+//     (6.6 TB/s); 1024 queries x 32 of 4096 lists, 1M x 1024 8-bit rows 186 us (5.5);
 //     4096 x 16 of 4096 lists, 1M x 768 bf16 rows 257 us (5.9; partly filled tiles cost
 //     the MMA warp as much as full ones, and a tile of 8-bit rows has fewer bytes).
 //   many queries: the operands through L2, 46 KB for 128 bytes of K of a 128 x 240 tile
@@ -64,22 +64,23 @@ constexpr int kItems = 8;               // tiles queued ahead
 // The launch shapes: up to NT queries a tile.  Rows and queries have rings of their
 // own (kX and kQ stages of kSlices slices; two slices a stage where the rows are read
 // for few queries, as a stage costs the MMA warp some 400 cycles beside its MMAs).
-// With up to 32 queries the queries' ring is the deeper one: gathered rows of q come
-// from anywhere in L2.
-template <int NT>
+// Lists of up to 32 queries a tile take a fifth stage of rows, as many of their tiles
+// are partly filled (1024 x 32 of 4096 lists 185 us for 191); the dense form measured
+// better with four (158 us for 168, one query against 1M rows).
+template <int NT, bool GROUP>
 struct Shape;
-template <>
-struct Shape<32> {
-    static constexpr int kX = 4, kQ = 8, kSlices = 2, kBox = 16, kAcc = 32, kTmem = 128,
-                         kSf = 4, kSf0 = 64, kSfStep = 8;
+template <bool GROUP>
+struct Shape<32, GROUP> {
+    static constexpr int kX = GROUP ? 5 : 4, kQ = GROUP ? 6 : 8, kSlices = 2, kBox = 16,
+                         kAcc = 32, kTmem = 128, kSf = 4, kSf0 = 64, kSfStep = 8;
 };
-template <>
-struct Shape<64> {
+template <bool GROUP>
+struct Shape<64, GROUP> {
     static constexpr int kX = 4, kQ = 4, kSlices = 2, kBox = 16, kAcc = 64, kTmem = 256,
                          kSf = 4, kSf0 = 128, kSfStep = 8;
 };
-template <>
-struct Shape<240> {  // each accumulator's scales in the 16 columns behind it
+template <bool GROUP>
+struct Shape<240, GROUP> {  // each accumulator's scales in the 16 columns behind it
     static constexpr int kX = 4, kQ = 4, kSlices = 1, kBox = 48, kAcc = 256, kTmem = 512,
                          kSf = 2, kSf0 = 240, kSfStep = 256;
 };
@@ -90,17 +91,18 @@ struct Item {
     int64_t j0;      // the first row's place in its list
 };
 
-template <int NT>
+template <int NT, bool GROUP>
 struct alignas(1024) Smem {
-    unsigned char x[Shape<NT>::kX][Shape<NT>::kSlices][kXBytes];
-    unsigned char q[Shape<NT>::kQ][Shape<NT>::kSlices][NT * kSlice];
+    using S = Shape<NT, GROUP>;
+    unsigned char x[S::kX][S::kSlices][kXBytes];
+    unsigned char q[S::kQ][S::kSlices][NT * kSlice];
     int64_t at[kItems][NT];  // where each column's scores start; -1: nowhere
     alignas(16) int32_t row[kItems][NT];  // each column's row of q (0 where there is none)
     int64_t prefix[kThreads + 1];
     Item items[kItems];
-    uint64_t xfull[Shape<NT>::kX], xempty[Shape<NT>::kX];
-    uint64_t qfull[Shape<NT>::kQ], qempty[Shape<NT>::kQ];
-    uint64_t accfull[2], accempty[2], sffull[Shape<NT>::kSf], sfempty[Shape<NT>::kSf];
+    uint64_t xfull[S::kX], xempty[S::kX];
+    uint64_t qfull[S::kQ], qempty[S::kQ];
+    uint64_t accfull[2], accempty[2], sffull[S::kSf], sfempty[S::kSf];
     uint64_t itemfull[kItems], itemempty[kItems], drain;
     int64_t warp_sum[kThreads / 32];
     uint32_t tmem;
@@ -295,9 +297,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap map_x32,
                      const __grid_constant__ CUtensorMap map_q, O* __restrict__ out,
                      const __grid_constant__ Params p) {
-    using S = Shape<NT>;
+    using S = Shape<NT, GROUP>;
+    // (a gathering warp meets its stages' slots at least a round apart: its waits by
+    // parity would not tell rounds apart otherwise)
+    static_assert(S::kQ >= kQueryWarps, "");
     extern __shared__ unsigned char smem_raw[];
-    Smem<NT>& sm = *reinterpret_cast<Smem<NT>*>(
+    auto& sm = *reinterpret_cast<Smem<NT, GROUP>*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -805,7 +810,7 @@ void row_map(CUtensorMap* m, const m3g_rows& r, int box_rows) {
 template <bool F8, int NT, bool GROUP, class O>
 cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* out,
                    unsigned grid, cudaStream_t st) {
-    constexpr size_t smem = sizeof(Smem<NT>) + 1024;
+    constexpr size_t smem = sizeof(Smem<NT, GROUP>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     auto kernel = scores_tc_kernel<F8, NT, GROUP, O>;
     // once a device (a bit each; devices past 64 set it every time)
@@ -822,7 +827,7 @@ cudaError_t launch(const m3g_rows& q, const m3g_rows& x, const Params& p, void* 
     CUtensorMap mx, mx32, mq;
     row_map(&mx, x, kM);
     row_map(&mx32, x, 32);
-    row_map(&mq, q, Shape<NT>::kBox);
+    row_map(&mq, q, Shape<NT, GROUP>::kBox);
     kernel<<<grid, kThreads, smem, st>>>(mx, mx32, mq, static_cast<O*>(out), p);
     return cudaGetLastError();
 }
