@@ -85,6 +85,25 @@ struct Shape<240, GROUP> {  // each accumulator's scales in the 16 columns behin
                          kSf = 2, kSf0 = 240, kSfStep = 256;
 };
 
+template <bool GROUP>
+struct Shape<112, GROUP> {  // many queries, bf16 rows and fp32 scores: see parts_of
+    static constexpr int kX = 6, kQ = 6, kSlices = 1, kBox = 56, kAcc = 112, kTmem = 256,
+                         kSf = 2, kSf0 = 224, kSfStep = 16;
+};
+
+// Accumulators a tile.  The tensor core cuts a sum's low bits where it could round, once
+// a MMA, so a sum of K dims comes out low by about K 2^-30 of itself for bf16 products
+// (K 2^-34 for e4m3 ones, whose sums seldom need the bits): 1e-6 at 1024 dims, 2.1e-6 at
+// 2048, where fp32 sums are within 4e-7.  fp32 scores of bf16 rows are added up from
+// sums of every fourth slice (4.7e-7 at 2048 dims).  With many queries that costs width:
+// 240 queries a tile have room for one sum, 112 for two, and L2 then gives the rows
+// twice (4096 x 16384 x 768: 147 us for 95), so the width goes by the dims: one sum up to
+// 512 (4.7e-7), two up to 1536 (7.2e-7), 64 queries with four above.
+template <bool F8, int NT, class O>
+constexpr int parts_of() {
+    return F8 || sizeof(O) != 4 || NT == 240 ? 1 : NT == 112 ? 2 : 4;
+}
+
 struct Item {
     int32_t x0, nx;  // first row of x, rows (0: no more tiles)
     int32_t q0, nq;  // first pair, pairs
@@ -203,6 +222,22 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
                  : "memory");
 }
 
+// 16 columns of the warp's TMEM lanes, added up over the first n of P accumulators that
+// are `step` columns apart.
+template <int P>
+__device__ __forceinline__ void tmem_ld16_sum(uint32_t taddr, int step, int n, uint32_t (&r)[16]) {
+    tmem_ld16(taddr, r);
+#pragma unroll
+    for (int a = 1; a < P; ++a) {
+        if (a >= n) break;
+        uint32_t s[16];
+        tmem_ld16(taddr + (uint32_t)(a * step), s);
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            r[u] = __float_as_uint(__uint_as_float(r[u]) + __uint_as_float(s[u]));
+    }
+}
+
 // Every other 16 of a tile's nq columns, from 16 * half on: a lane stores its row's
 // score of column c at mine[c * ld].  The next columns are on their way from TMEM while
 // these are stored (a load waited for at once, and a multiplication for each address,
@@ -258,8 +293,8 @@ struct Tiles {
         }
         per = (int32_t)max((n + 15u) & ~15u, 16u);
         nqt = n == (uint32_t)m ? 1 : (int32_t)(((uint32_t)m + per - 1) / (uint32_t)per);
-        w = NT > 128 ? 1 : 9;
-        wlast = NT > 128 ? 1 : 1 + 2 * ((int32_t)(len - (nx - 1) * kM) + 31) / 32;
+        w = NT > 64 ? 1 : 9;
+        wlast = NT > 64 ? 1 : 1 + 2 * ((int32_t)(len - (nx - 1) * kM) + 31) / 32;
     }
     __device__ __forceinline__ int64_t count() const { return nx * nqt; }
     __device__ __forceinline__ int64_t weight() const {
@@ -306,7 +341,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (warp == 0) tmem_alloc(&sm.tmem, S::kTmem);
+    constexpr int P = parts_of<F8, NT, O>();
+    constexpr int kAcc = P > 1 ? P * NT : S::kAcc;  // columns from one tile's to the next's
+    constexpr int kTmem = P == 1 ? S::kTmem : 2 * kAcc > 256 ? 512 : 256;
+    static_assert(P == 1 || 2 * kAcc <= 512, "");
+    static_assert(!F8 || NT != 112, "");
+    if (warp == 0) tmem_alloc(&sm.tmem, kTmem);
     if (threadIdx.x == 32) {
         for (int s = 0; s < S::kX; ++s) {
             mbar_init(&sm.xfull[s], 1);
@@ -529,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                    &sm.abort)))
                 break;
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(h * S::kAcc);
+            const uint32_t d = tmem + (uint32_t)(h * kAcc);
             const uint32_t idesc = F8 ? mx_idesc(n) : tc_idesc_m128(n, 1);
             for (int kt = 0; kt < p.nk; kt += S::kSlices) {
                 const bool first = F8 && (kt & 3) == 0;
@@ -551,8 +591,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             dx0 + (rx.i * S::kSlices + s) * (kXBytes >> 4) + 2 * k;
                         const uint64_t b =
                             dq0 + (rq.i * S::kSlices + s) * (NT * kSlice >> 4) + 2 * k;
-                        if (F8) tc_mma_mx(d, a, b, id, tsf, tsf + 4, (kt | s | k) != 0);
-                        else tc_mma_f16(d, a, b, id, (kt | s | k) != 0);
+                        const uint32_t to = d + (uint32_t)((kt + s) % P * NT);
+                        const bool more = kt + s >= P || k > 0;
+                        if (F8) tc_mma_mx(to, a, b, id, tsf, tsf + 4, more);
+                        else tc_mma_f16(to, a, b, id, more);
                     };
 #pragma unroll
                     for (int s = 0; s < S::kSlices; ++s) {
@@ -760,19 +802,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
             const uint32_t acc =
-                tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(h * S::kAcc);
+                tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(h * kAcc);
             if (quarter * 32 < item.nx) {
                 const bool in = row < item.nx;
-                if constexpr (GROUP) {
+                if constexpr (GROUP || P > 1) {
                     const int64_t* at = sm.at[i % kItems];
 #pragma unroll 1
                     for (int c0 = 16 * half; c0 < item.nq; c0 += 32) {
                         uint32_t r[16];
-                        tmem_ld16(acc + (uint32_t)c0, r);
+                        tmem_ld16_sum<P>(acc + (uint32_t)c0, NT, p.nk, r);
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
                             if (c0 + u >= item.nq) break;
-                            const int64_t o = at[c0 + u];
+                            const int64_t o = GROUP ? at[c0 + u]
+                                                    : (item.q0 + c0 + u) * p.ld_out + item.j0;
                             if (in && o >= 0)
                                 put_score(out + o + row,
                                           fmaf(p.alpha, __uint_as_float(r[u]), p.beta));
@@ -795,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, S::kTmem);
+        tmem_dealloc(tmem, kTmem);
     }
 }
 
@@ -838,14 +881,19 @@ cudaError_t launch_any(const m3g_rows& q, const m3g_rows& x, const Params& p, in
     const bool f32 = out_dtype == M3G_F32;
     auto with = [&](auto nt) {
         constexpr int NT = decltype(nt)::value;
-        if (x.dtype == M3G_E4M3)
+        if constexpr (NT == 112)
+            return launch<false, NT, GROUP, float>(q, x, p, out, grid, st);
+        else if (x.dtype == M3G_E4M3)
             return f32 ? launch<true, NT, GROUP, float>(q, x, p, out, grid, st)
                        : launch<true, NT, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
-        return f32 ? launch<false, NT, GROUP, float>(q, x, p, out, grid, st)
-                   : launch<false, NT, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
+        else
+            return f32 ? launch<false, NT, GROUP, float>(q, x, p, out, grid, st)
+                       : launch<false, NT, GROUP, __nv_bfloat16>(q, x, p, out, grid, st);
     };
     if (queries <= 32) return with(std::integral_constant<int, 32>());
-    if (queries <= 64) return with(std::integral_constant<int, 64>());
+    const bool sums = f32 && x.dtype == M3G_BF16;
+    if (queries <= 64 || (sums && x.dim > 1536)) return with(std::integral_constant<int, 64>());
+    if (sums && x.dim > 512) return with(std::integral_constant<int, 112>());
     return with(std::integral_constant<int, 240>());
 }
 

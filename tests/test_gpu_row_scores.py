@@ -194,6 +194,24 @@ def test_row_scores_into_strided_output(R, eng, kind, out_dtype, off):
     assert (rest == 7.0).all()
 
 
+@pytest.mark.parametrize("dim", [96, 512, 513, 1024, 1536, 1537, 2048, 4000])
+@pytest.mark.parametrize("nq", [1, 40, 300])
+def test_fp32_scores_of_bf16_rows_are_not_low(R, eng, dim, nq):
+    """Sums of like terms (a query and rows near one another): the tensor core cuts sums at every
+    16 dims, by half a step of fp32 each on average; sums of a quarter (from 1537 dims on, or with
+    up to 64 queries), half (from 513) or all of the dims keep what is lost below dim / 16 / parts
+    half steps of 2^-23, and fp32 rounding of the parts' sum below two more."""
+    base = randn(1, dim, seed=dim)
+    x = (base + 0.3 * randn(2000, dim, seed=1)).bfloat16()
+    q = (base + 0.3 * randn(nq, dim, seed=2)).bfloat16()
+    st = lambda v: torch.nn.functional.pad(v, (0, -dim % 8))[:, :dim]  # noqa: E731
+    got = R.row_scores(eng, st(q), st(x)).double()
+    want = q.double() @ x.double().t()
+    parts = 4 if nq <= 64 or dim > 1536 else 2 if dim > 512 else 1
+    low = ((want - got) / want).mean().item()
+    assert abs(low) <= (dim / 16 / parts / 2 + 2) * 2 * U32, low
+
+
 def test_row_scores_nan_rows(R, eng):
     """A NaN in one row reaches that row's scores alone, whatever the neighbours in its tile are;
     rows past the last one are not read into anything."""
