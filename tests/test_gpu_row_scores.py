@@ -303,7 +303,11 @@ LISTS = [  # nlist, mean rows, queries, dim, pairs per list
     (12, 200, 300, 200, lambda r, g: int(r.choice([0, 1, 15, 16, 17, 63, 64, 65, 240, 241, 300]))),
     (700, 20, 64, 64, lambda r, g: int(r.random() < 0.5)),
     (300, 64, 100, 130, lambda r, g: int(r.integers(0, 4))),
-    (3, 3000, 20, 96, lambda r, g: 5), (2500, 3, 64, 128, lambda r, g: int(r.integers(0, 3)))]
+    (3, 3000, 20, 96, lambda r, g: 5), (2500, 3, 64, 128, lambda r, g: int(r.integers(0, 3))),
+    (9, 150, 40, 48, lambda r, g: int(r.choice([0, 33, 40, 48, 64, 90]))),
+    (8, 150, 200, 640, lambda r, g: int(r.choice([0, 100, 111, 112, 113, 200]))),
+    (9, 150, 40, 1030, lambda r, g: int(r.choice([0, 33, 40, 48, 64, 90]))),
+    (8, 150, 200, 1600, lambda r, g: int(r.choice([0, 64, 65, 100, 129, 200])))]
 
 
 @pytest.mark.parametrize("i", range(len(LISTS)))
