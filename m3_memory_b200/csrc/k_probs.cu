@@ -11,8 +11,8 @@
 //
 // A warp takes a row, or one of P parts of it where rows are few, on its own: no warp
 // waits for another, and one's latencies (row offsets, the final order, the outputs)
-// pass behind the others' work.  Its scores come through a ring of three 4 KB bulk
-// copies, so 144 KB an SM are in flight whatever the warps do.  Parts leave (m, z, w)
+// pass behind the others' work.  Its scores come through a ring of two 4 KB bulk
+// copies, so 160 KB an SM are in flight whatever the warps do.  Parts leave (m, z, w)
 // and their best k in the caller's scratch and a second kernel joins them.
 //
 // The best k pass through a buffer of the warp's: entries that reach the bound tau, a
@@ -101,7 +101,8 @@ __device__ __forceinline__ void rebase(Sums& s, float c, float m) {
         s.m = m;
         return;
     }
-    const float d = fmaxf(c * s.m - c * m, -1000.f), f = exp_of(d);
+    // (the products as rounded, not fused into the difference: z and w refer to them)
+    const float d = fmaxf(__fmul_rn(c, s.m) - __fmul_rn(c, m), -1000.f), f = exp_of(d);
     s.w = f * fmaf(d, s.z, s.w);
     s.z *= f;
     s.m = m;
@@ -300,7 +301,7 @@ template <class T>
 __device__ __forceinline__ void finish_row(const ProbsArgs& a, int64_t row, const RowAt& at,
                                            const Sums& s, const unsigned long long* keys,
                                            int kept, float c, float sgn, int tid, int threads) {
-    const float cm = s.m > ninf() ? c * s.m : ninf();
+    const float cm = s.m > ninf() ? __fmul_rn(c, s.m) : ninf();
     const bool inf = cm == __int_as_float(0x7f800000);
     const float logz = logf(s.z);
     if (tid == 0) {
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
             m = fmaxf(m, hm);
             if (hm >= a.lowest) {
                 if (hm > s.m) rebase(s, c, hm);
-                const float cm = c * s.m;
+                const float cm = __fmul_rn(c, s.m);
                 const uint64_t cc = pack2(c, c), mm = pack2(-cm, -cm);
                 const uint64_t l2 = pack2(1.4426950408889634f, 1.4426950408889634f);
                 uint64_t z = 0, w = 0;
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
             const float t[1] = {__uint_as_float(__float_as_uint(edge) ^ flip)};
             if (t[0] >= a.lowest) {
                 if (t[0] > s.m) rebase(s, c, t[0]);
-                const float d = fmaxf(fmaf(c, t[0], -(c * s.m)), -1000.f), e = exp_of(d);
+                const float d = fmaxf(fmaf(c, t[0], -__fmul_rn(c, s.m)), -1000.f), e = exp_of(d);
                 s.z += e;
                 s.w = fmaf(e, d, s.w);
             }
