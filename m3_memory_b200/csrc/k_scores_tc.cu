@@ -653,8 +653,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int u = 0; u < W - 4; ++u) {
                     const int c = lane + 32 * u;
-                    const int64_t r = gather ? (c < item.nq ? sm.row[i % kItems][c] : 0)
-                                             : (int64_t)item.q0 + c;
+                    // (the queued row: a pair that is out of range has row 0)
+                    const int64_t r = GROUP ? (c < item.nq ? sm.row[i % kItems][c] : 0)
+                                            : (int64_t)item.q0 + c;
                     ptr[4 + u] = c < item.nq ? p.qs + r * p.lqs : nullptr;
                 }
                 done_with(i++);
