@@ -701,10 +701,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = mbar_wait(&sm.itemempty[s], (uint32_t)((i / kItems) - 1) & 1u, &sm.abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
-            if constexpr (F8) {  // the rows' scale words, into L2 before they are read
+            if constexpr (F8) {
+                // the rows' scale words, into L2 before they are read: a range where lines
+                // hold several rows', row by row where what lies between is not theirs
                 const uint8_t* b = p.xs + (int64_t)item.x0 * p.lxs;
-                for (int64_t o = 128 * lane; o < item.nx * p.lxs; o += 128 * 32)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
+                auto prefetch = [](const uint8_t* at) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                };
+                if (p.lxs <= 128) {
+                    const int n = (item.nx - 1) * (int)p.lxs + p.nk;
+                    for (int o = 128 * lane; o < n; o += 128 * 32) prefetch(b + o);
+                } else {
+                    for (int r = lane; r < item.nx; r += 32)
+                        for (int o = 0; o < p.nk; o += 128) prefetch(b + r * p.lxs + o);
+                }
             }
             if constexpr (GROUP) {
                 for (int c = lane; c < columns(item); c += 32) {

@@ -45,3 +45,47 @@ def test_more_pairs_than_queries_without_pair_row(R, eng, kind, npair):
     got = out.view(npair, length)
     assert ((got[:nq].double() - ref).abs() <= tol).all()
     assert (got[nq:] == 7.0).all()
+
+
+# ---------------- wide strides ----------------
+
+
+def spread(p, dim, codes_ld, scales_ld):
+    """The same packed rows with other row strides."""
+    n = p.codes.shape[0]
+    codes = torch.empty(n, codes_ld, dtype=torch.uint8, device="cuda")[:, :p.codes.shape[1]]
+    scales = torch.empty(n, scales_ld, dtype=torch.uint8, device="cuda")[:, :p.scales.shape[1]]
+    codes.copy_(p.codes)
+    scales.copy_(p.scales)
+    return type(p)(codes, scales, dim)
+
+
+@pytest.mark.parametrize("n,dim,scales_ld", [(130, 600, 1 << 24), (1000, 640, 1 << 18),
+                                             (300, 520, 132), (257, 17000, 256)])
+def test_scales_far_apart(R, eng, n, dim, scales_ld):
+    """Scale bytes that are a small part of wider records: only they are touched, and the records'
+    size costs nothing (walking all of 130 x 16 MB would outlast the waits' limit)."""
+    x = R.pack_rows(eng, torch.randn(n, dim, device="cuda"))
+    q = R.pack_rows(eng, torch.randn(20, dim, device="cuda"))
+    want = R.row_scores(eng, q, x)
+    wide = spread(x, dim, -(-dim // 16) * 16 + 16, scales_ld)
+    assert torch.equal(R.row_scores(eng, q, wide), want)
+    assert torch.equal(R.row_scores(eng, spread(q, dim, -(-dim // 16) * 16, scales_ld), x), want)
+    out = torch.empty(20 * n, device="cuda")
+    R.list_scores(eng, q, wide, T([0]), T([n], torch.int32), T([0, 20]),
+                  torch.arange(20, device="cuda") * n, out)
+    assert torch.equal(out.view(20, n), want)
+    eng.sync_errors()
+
+
+def test_codes_and_scales_in_one_record(R, eng):
+    """Records of a row's codes and its scales behind them, the last row's scales at the end."""
+    n, dim = 300, 1024
+    p = R.pack_rows(eng, torch.randn(n, dim, device="cuda"))
+    rec = torch.empty(n, dim + 16, dtype=torch.uint8, device="cuda")
+    rec[:, :dim], rec[:, dim:dim + 8] = p.codes, p.scales
+    x = R.PackedRows(rec[:, :dim], rec[:, dim:dim + 8], dim)
+    for nq in (1, 100):
+        q = R.pack_rows(eng, torch.randn(nq, dim, device="cuda"))
+        assert torch.equal(R.row_scores(eng, q, x), R.row_scores(eng, q, p))
+    eng.sync_errors()
