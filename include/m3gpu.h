@@ -406,8 +406,9 @@ int m3g_list_scores_device(m3g_engine* e, const m3g_rows* q, const m3g_rows* x, 
  * d_row_off[i] .. d_row_off[i + 1] - 1 of n entries in all (ld is not used; a row out
  * of range is taken as one without entries, and reported).  A row holds at most
  * 2^31 - 2^16 entries.  With
- * l = scale * score (scale finite and not 0), over the entries whose l is neither
- * NaN nor -inf (the others are left out: they have no probability):
+ * l = scale * score (scale finite and not 0; infinite past fp32's range), over the
+ * entries whose l is neither NaN nor -inf (the others are left out: they have no
+ * probability):
  *   out_logsumexp[i] = log sum exp(l)               (-inf where no entry is left)
  *   out_entropy[i]   = -sum p log p, p = exp(l - logsumexp)   (0 there)
  *   out_given[i, j]  = log p of entry d_given[i, j] (its place in the row) of ngiven

@@ -6,8 +6,11 @@
 // d = c t - c m.  Parts join by M = max m, z' = e^(c m - c M) z and
 // w' = e^(c m - c M) (w + (c m - c M) z); then logsumexp = c M + log z and
 // entropy = log z - w / z.  d is one fma on c m as rounded, so the formulas hold
-// exactly whatever that rounding was.  Entries that are NaN, or -inf after scaling,
-// come out of max(d, -1000) with e^d = 0; a.lowest is the least t that is neither.
+// exactly whatever that rounding was, as long as e^(what it cut off) is near one: a part
+// whose |c m| is 2^24 or more is summed up again from c m in two words (ref_of; in the
+// first pass the second word cost 3% of every row's time).  Entries that are NaN, or
+// -inf after scaling, come out of max(d, -1000) with e^d = 0; a.lowest is the least t
+// that is neither.
 //
 // A warp takes a row, or one of P parts of it where rows are few, on its own: no warp
 // waits for another, and one's latencies (row offsets, the final order, the outputs)
@@ -95,16 +98,36 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// a part's sums taken to another reference value
+// The value hi + lo that a part's z and w refer to: c m as rounded (not fused into what
+// it is subtracted from) and, where that may be off by 1/2 and more, what the rounding
+// cut off (exact).  With hi alone, at c m = 3e9, the largest entry's e^d could be e^128.
+struct Ref {
+    float hi, lo;
+};
+__device__ __forceinline__ Ref ref_of(float c, float m) {
+    const float hi = __fmul_rn(c, m), a = fabsf(hi);
+    return {hi, a >= 16777216.f && a < __int_as_float(0x7f800000) ? fmaf(c, m, -hi) : 0.f};
+}
+// c t less the reference value.  Next to a c m that was rounded by lo there are no
+// entries nearer than lo / 2, so the two roundings are within 2^-22 of the result.
+__device__ __forceinline__ float from_ref(float c, float t, const Ref& ref) {
+    return fmaf(c, t, -ref.hi) - ref.lo;
+}
+
+// a part's sums taken to another reference value; LO: of two words
+template <bool LO = true>
 __device__ __forceinline__ void rebase(Sums& s, float c, float m) {
     if (s.m == m || s.z == 0.f) {
         s.m = m;
         return;
     }
-    // (the products as rounded, not fused into the difference: z and w refer to them)
-    const float d = fmaxf(__fmul_rn(c, s.m) - __fmul_rn(c, m), -1000.f), f = exp_of(d);
-    s.w = f * fmaf(d, s.z, s.w);
-    s.z *= f;
+    float d = __fmul_rn(c, s.m) - __fmul_rn(c, m);
+    if (LO) d += ref_of(c, s.m).lo - ref_of(c, m).lo;
+    d = fmaxf(d, -1000.f);
+    const float f = exp_of(d);
+    // (where f is 0, z may be infinite: see ref_of)
+    s.w = f > 0.f ? f * fmaf(d, s.z, s.w) : 0.f;
+    s.z = f > 0.f ? s.z * f : 0.f;
     s.m = m;
 }
 __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
@@ -117,11 +140,12 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
 }
 
 // The sums of all lanes, in fixed order, in every lane.
+template <bool LO = true>
 __device__ __forceinline__ Sums warp_join(Sums s, float c) {
     float m = s.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    rebase(s, c, m);
+    rebase<LO>(s, c, m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
@@ -288,11 +312,12 @@ __device__ __forceinline__ RowAt row_at(const ProbsArgs& a, int64_t row) {
 }
 
 // l = c t, or the reference value where that is infinite
-__device__ __forceinline__ float log_prob(float t, float c, float cm, float logz) {
+__device__ __forceinline__ float log_prob(float t, float c, const Ref& ref, float logz) {
     const float l = c * t;
     if (!(l > ninf())) return ninf();  // left out
-    if (cm == __int_as_float(0x7f800000)) return l == cm ? __int_as_float(0x7fc00000) : ninf();
-    return fmaf(c, t, -cm) - logz;
+    if (ref.hi == __int_as_float(0x7f800000))
+        return l == ref.hi ? __int_as_float(0x7fc00000) : ninf();
+    return from_ref(c, t, ref) - logz;
 }
 
 // The answer of a row from its sums and its best entries (keys, sorted, kept of them),
@@ -301,11 +326,11 @@ template <class T>
 __device__ __forceinline__ void finish_row(const ProbsArgs& a, int64_t row, const RowAt& at,
                                            const Sums& s, const unsigned long long* keys,
                                            int kept, float c, float sgn, int tid, int threads) {
-    const float cm = s.m > ninf() ? __fmul_rn(c, s.m) : ninf();
-    const bool inf = cm == __int_as_float(0x7f800000);
+    const Ref ref = s.m > ninf() ? ref_of(c, s.m) : Ref{ninf(), 0.f};
+    const bool inf = ref.hi == __int_as_float(0x7f800000);
     const float logz = logf(s.z);
     if (tid == 0) {
-        a.lse[row] = inf || !(s.z > 0.f) ? cm : cm + logz;
+        a.lse[row] = inf || !(s.z > 0.f) ? ref.hi : ref.hi + (ref.lo + logz);
         a.entropy[row] = inf          ? __int_as_float(0x7fc00000)
                          : s.z > 0.f ? fmaxf(logz - s.w / s.z, 0.f)  // (roundings aside)
                                      : 0.f;
@@ -314,12 +339,12 @@ __device__ __forceinline__ void finish_row(const ProbsArgs& a, int64_t row, cons
     for (int j = tid; j < a.ngiven; j += threads) {
         const int64_t g = a.given[row * a.ngiven + j];
         a.out_given[row * a.ngiven + j] =
-            g >= 0 && g < at.len ? log_prob(sgn * load_score(x + g), c, cm, logz) : ninf();
+            g >= 0 && g < at.len ? log_prob(sgn * load_score(x + g), c, ref, logz) : ninf();
     }
     for (int j = tid; j < a.k; j += threads) {
         const unsigned long long key = j < kept ? keys[j] : kNone;
         a.top_index[row * a.k + j] = key == kNone ? -1 : (int64_t)(uint32_t)key;
-        a.top[row * a.k + j] = key == kNone ? ninf() : log_prob(t_of(key), c, cm, logz);
+        a.top[row * a.k + j] = key == kNone ? ninf() : log_prob(t_of(key), c, ref, logz);
     }
 }
 
@@ -620,7 +645,7 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
             }
             m = fmaxf(m, hm);
             if (hm >= a.lowest) {
-                if (hm > s.m) rebase(s, c, hm);
+                if (hm > s.m) rebase<false>(s, c, hm);
                 const float cm = __fmul_rn(c, s.m);
                 const uint64_t cc = pack2(c, c), mm = pack2(-cm, -cm);
                 const uint64_t l2 = pack2(1.4426950408889634f, 1.4426950408889634f);
@@ -688,14 +713,28 @@ __global__ void __launch_bounds__(warps_of(KW) * 32, 1)
         if (__any_sync(0xffffffffu, edge == edge)) {
             const float t[1] = {__uint_as_float(__float_as_uint(edge) ^ flip)};
             if (t[0] >= a.lowest) {
-                if (t[0] > s.m) rebase(s, c, t[0]);
+                if (t[0] > s.m) rebase<false>(s, c, t[0]);
                 const float d = fmaxf(fmaf(c, t[0], -__fmul_rn(c, s.m)), -1000.f), e = exp_of(d);
                 s.z += e;
                 s.w = fmaf(e, d, s.w);
             }
             if (a.k > 0) offer(t, edge_at);
         }
-        s = warp_join(s, c);
+        s = warp_join<false>(s, c);
+        const Ref ref = ref_of(c, s.m);
+        if (ref.lo != 0.f) {  // (the same in every lane)
+            s.z = s.w = 0.f;
+            auto add = [&](float t) {
+                const float d = fmaxf(from_ref(c, t, ref), -1000.f), e = exp_of(d);
+                s.z += e;
+                s.w = fmaf(e, d, s.w);
+            };
+            const T* at = x + u.head + (int64_t)u.g0 * V;
+            const int m = (u.g1 - u.g0) * V;
+            for (int i = lane; i < m; i += 32) add(sgn * load_score(at + i));
+            add(sgn * edge);
+            s = warp_join<false>(s, c);
+        }
         int kept = 0;
         if (a.k > 0) kept = cut<KW>(sm.buf, keys, n, a.k);
         if (parts == 1) {

@@ -1,11 +1,13 @@
 """Row scores at the limits of what a call may be given."""
+import numpy as np
 import pytest
 import torch
 
 from m3_memory_b200 import cabi
-from test_gpu_row_scores import make_rows, scores_ref
+from test_gpu_row_scores import close, make_rows, probs_check, scores_ref
 
 pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24  # half a step of fp32, relative
 
 
 @pytest.fixture(scope="module")
@@ -89,3 +91,87 @@ def test_codes_and_scales_in_one_record(R, eng):
         q = R.pack_rows(eng, torch.randn(nq, dim, device="cuda"))
         assert torch.equal(R.row_scores(eng, q, x), R.row_scores(eng, q, p))
     eng.sync_errors()
+
+
+# ---------------- large logits ----------------
+
+
+def near_equal(nq, n, size, dtype, seed):
+    """Scores within a few steps of their type below `size` (whose products with a scale fp32
+    rounds by many units), a few far below, some left out."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    step = size * torch.finfo(dtype).eps
+    s = size - step * torch.randint(0, 6, (nq, n), device="cuda", generator=g)
+    s[torch.rand(nq, n, device="cuda", generator=g) < 0.3] *= -0.5
+    s[torch.rand(nq, n, device="cuda", generator=g) < 0.05] = float("nan")
+    s[torch.rand(nq, n, device="cuda", generator=g) < 0.05] = -float("inf")
+    return s.to(dtype)
+
+
+@pytest.mark.parametrize("nq,n,k", [(3, 1, 1), (2, 7, 3), (5, 1000, 10), (4, 5003, 100),
+                                    (2, 100003, 10), (300, 777, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size,scale", [(3e8, 50.3), (-3e8, 50.3), (1e6, 1.7), (2.5e4, 50.3),
+                                        (1e9, 7.7), (1e30, 1.1), (4e7, 1e20), (1.2e10, -0.3)])
+def test_large_logits(R, eng, nq, n, k, dtype, size, scale):
+    """Logits far past 2^20, where fp32 rounds the largest one by more than e^x bears."""
+    s = near_equal(nq, n, size, dtype, nq + n) * (1.0 if scale > 0 else -1.0)
+    # the formula's scale is the fp32 value; a product of it with a score is exact in 64 bits
+    given = torch.randint(-1, n + 1, (nq, 2), device="cuda")
+    rows, scale = list(s.float().cpu().numpy()), float(np.float32(scale))
+    probs_check(R, eng, s, rows, scale, k, given)
+    # log p again, without the largest logit's size in the tolerance: l - m is exact to 2^-22 of
+    # itself, log z to the relative error of z (see probs_ref), the difference to half a step
+    got = R.score_probs(eng, s, scale=scale, k=k, given=given)
+    for i, r in enumerate(rows):
+        l = np.asarray(r, np.float64) * scale
+        held = l > -np.inf
+        if not held.any():
+            continue
+        d = np.where(held, l - l[held].max(), -np.inf)
+        p = np.exp(d)
+        z, x = p.sum(), -(p * np.where(held, d, 0.0)).sum()
+        e_z = (n / 256 + 40) * U32 + 2.0 ** -21 + 2.0 ** -22 * x / z
+        pairs = [(got.given[i].cpu().numpy(),
+                  [d[j] if 0 <= j < n else -np.inf for j in given[i].tolist()])]
+        if k:
+            at = got.top_index[i].cpu().numpy()
+            pairs.append((got.top[i].cpu().numpy()[at >= 0], d[at[at >= 0]]))
+        for have, want in pairs:
+            want = np.asarray(want)
+            dist = np.abs(np.nan_to_num(want, neginf=0.0))
+            logp = want - np.log(z)
+            tol = e_z + 4 * U32 * dist + 4 * U32 * (dist + abs(np.log(z)))
+            assert close(have, logp, tol), (i, have, logp, tol)
+
+
+def test_large_logits_ragged(R, eng):
+    size = [0, 1, 40, 9000, 3, 20011]
+    off = T(size).cumsum(0)
+    off = torch.cat([T([0]), off])
+    s = near_equal(1, sum(size), 3e8, torch.float32, 5)[0]
+    f = s.cpu().numpy()
+    rows = [f[a:b] for a, b in zip(off.tolist(), off.tolist()[1:])]
+    probs_check(R, eng, s, rows, float(np.float32(50.3)), 12, row_off=off)
+
+
+@pytest.mark.parametrize("mask", [-1e9, -3e4, -1e30, torch.finfo(torch.float32).min,
+                                  torch.finfo(torch.bfloat16).min])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [50.3, 0.7])
+def test_rows_masked_by_a_large_value(R, eng, mask, dtype, scale):
+    """Entries masked by a large finite value instead of -inf: runs of them at the start, at the
+    end, whole parts of a long row, and rows of nothing else."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    scale = float(np.float32(scale))
+    for nq, n, k in ((6, 9000, 10), (4, 60001, 100)):
+        s = torch.randn(nq, n, device="cuda", generator=g)
+        s[0, :n // 2] = mask
+        s[1, n // 3:] = mask
+        s[2] = mask
+        s[3, torch.rand(n, device="cuda", generator=g) < 0.9] = mask
+        s = s.to(dtype)
+        rows = s.float().cpu().numpy()
+        # l is an fp32 value: a product below fp32's range is -inf, and such entries are left out
+        rows[rows.astype(np.float64) * scale < -3.4028235677973366e38] = -np.inf
+        probs_check(R, eng, s, list(rows), scale, k)
