@@ -108,6 +108,7 @@ struct Item {
     int32_t x0, nx;  // first row of x, rows (0: no more tiles)
     int32_t q0, nq;  // first pair, pairs
     int64_t j0;      // the first row's place in its list
+    int64_t len;     // rows of the list
 };
 
 template <int NT, bool GROUP>
@@ -725,8 +726,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int64_t pr = (int64_t)item.q0 + c;
                     const int64_t row = gather ? (int64_t)p.g.pair_row[pr] : pr;
                     const int64_t at = p.g.out_off[pr];
+                    // (by the whole list's length: a pair's tiles decide alike)
                     const bool in = row >= 0 && row < p.nq && at >= 0 &&
-                                    at <= p.g.out_n - (item.j0 + item.nx);
+                                    at <= p.g.out_n - item.len;
                     if (!in && row != -1) atomicOr(p.err + kScoreBadItem, 1);
                     sm.row[s][c] = in ? (int32_t)row : 0;
                     sm.at[s][c] = in ? at + item.j0 : -1;
@@ -752,6 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 Item item;
                 item.j0 = xt * kM;
+                item.len = at.len;
                 item.x0 = (int32_t)(at.l0 + item.j0);
                 item.nx = (int32_t)min((int64_t)kM, at.len - item.j0);
                 item.q0 = (int32_t)(at.p0 + (int64_t)qt * g.per);
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             queue_group(GroupAt{0, p.nx, 0, p.nq}, Tiles<NT>(p.nx, p.nq), blockIdx.x, total,
                         gridDim.x);
         }
-        if (ok) queue(Item{0, 0, 0, 0, 0});
+        if (ok) queue(Item{0, 0, 0, 0, 0, 0});
     } else if (warp >= kEpi0 && warp < kQuery0) {
         // ---- epilogue: warp w holds TMEM lanes 32 (w & 3) .. of the tile's rows, and
         // every other 16 columns

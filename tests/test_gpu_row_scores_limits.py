@@ -49,6 +49,33 @@ def test_more_pairs_than_queries_without_pair_row(R, eng, kind, npair):
     assert (got[nq:] == 7.0).all()
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "bf16"])
+@pytest.mark.parametrize("gather", [True, False])
+def test_pair_that_ends_past_the_output_is_left_out_whole(R, eng, kind, gather):
+    """A list of several tiles, written for one pair to the last elements, for others past them by
+    one or by more than a tile: none of their scores is written, before the end either."""
+    nq, n, dim, length = 4, 900, 192, 700
+    q, qv = make_rows(R, eng, kind, nq, dim, 1)
+    x, xv = make_rows(R, eng, kind, n, dim, 2)
+    out_n = 3 * length
+    out = torch.full((out_n,), 7.0, device="cuda")
+    start = [out_n - length, out_n - length + 1, length, out_n - 200]
+    R.list_scores(eng, q, x, T([150]), T([length], torch.int32), T([0, nq]), T(start), out,
+                  pair_row=T([0, 1, 2, 3], torch.int32) if gather else None)
+    with pytest.raises(IndexError):
+        eng.sync_errors()
+    ref, tol = scores_ref(qv, xv[150:150 + length], 1.0, 0.0, torch.float32, dim)
+    assert (out[:length] == 7.0).all()
+    assert ((out[length:2 * length].double() - ref[2]).abs() <= tol[2]).all()
+    assert ((out[2 * length:].double() - ref[0]).abs() <= tol[0]).all()
+    # alone: nothing at all
+    out.fill_(7.0)
+    R.list_scores(eng, q, x, T([150]), T([length], torch.int32), T([0, 1]), T(start[3:]), out)
+    with pytest.raises(IndexError):
+        eng.sync_errors()
+    assert (out == 7.0).all()
+
+
 # ---------------- wide strides ----------------
 
 
