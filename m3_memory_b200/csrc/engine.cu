@@ -812,7 +812,7 @@ void Engine::set_device(int dev) {
     if (dev < 0 || dev >= count) fail(M3G_EINVAL, "set_device: no such CUDA device");
     std::shared_lock lk(imu_);
     std::lock_guard sl(score_mu_);
-    if (!indices_.empty() || ws_.stream || score_err_.p)
+    if (!indices_.empty() || ws_.stream || score_err_.load())
         fail(M3G_ERUNTIME, "set_device: engine already in use");
     device_ = dev;
     int n = 0;

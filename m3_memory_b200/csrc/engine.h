@@ -351,11 +351,13 @@ class Engine {
     int first_error_code_ = 0;
 
     // error words of the row-score calls (kScoreErrWords ints on the device, made by
-    // the first call); row_score_errors() reads and clears them
+    // the first call, under score_mu_; later ones take no lock); row_score_errors()
+    // reads and clears them, one caller at a time
     int* score_err();
     void row_score_errors();
-    std::mutex score_mu_;
-    DBuf<int> score_err_;
+    std::mutex score_mu_, score_read_mu_;
+    DBuf<int> score_words_;
+    std::atomic<int*> score_err_{nullptr};  // score_words_, once they are cleared
 
     Workspace ws_;
     std::atomic<bool> profiling_{false};

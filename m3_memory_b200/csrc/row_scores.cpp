@@ -67,25 +67,27 @@ float lowest_score(float c) {
 }  // namespace
 
 int* Engine::score_err() {
+    if (int* words = score_err_.load()) return words;
     std::lock_guard lk(score_mu_);
-    if (!score_err_.p) {
+    if (!score_err_.load()) {
         DBuf<int> w;
         w.alloc(kScoreErrWords);
         M3G_CK(cudaMemset(w.p, 0, kScoreErrWords * sizeof(int)));
         M3G_CK(cudaStreamSynchronize(cudaStreamLegacy));
-        score_err_.swap(w);
+        score_words_.swap(w);
+        score_err_ = score_words_.p;
     }
-    return score_err_.p;
+    return score_err_.load();
 }
 
 void Engine::row_score_errors() {
-    std::lock_guard lk(score_mu_);
-    if (!score_err_.p) return;
+    int* words = score_err_.load();
+    if (!words) return;
+    std::lock_guard lk(score_read_mu_);
     M3G_CK(cudaDeviceSynchronize());
     int w[kScoreErrWords];
-    M3G_CK(cudaMemcpy(w, score_err_.p, sizeof(w), cudaMemcpyDeviceToHost));
-    if (w[kScoreTimeout] || w[kScoreBadItem])
-        M3G_CK(cudaMemset(score_err_.p, 0, sizeof(w)));
+    M3G_CK(cudaMemcpy(w, words, sizeof(w), cudaMemcpyDeviceToHost));
+    if (w[kScoreTimeout] || w[kScoreBadItem]) M3G_CK(cudaMemset(words, 0, sizeof(w)));
     if (w[kScoreTimeout]) fail(M3G_ETIMEOUT, "row scores: a device-side wait gave up");
     if (w[kScoreBadItem])
         fail(M3G_ERANGE, "row scores: a list, pair or row of scores out of range was left out");

@@ -1,4 +1,7 @@
 """Row scores at the limits of what a call may be given."""
+import threading
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -202,3 +205,35 @@ def test_rows_masked_by_a_large_value(R, eng, mask, dtype, scale):
         # l is an fp32 value: a product below fp32's range is -inf, and such entries are left out
         rows[rows.astype(np.float64) * scale < -3.4028235677973366e38] = -np.inf
         probs_check(R, eng, s, list(rows), scale, k)
+
+
+# ---------------- several callers ----------------
+
+
+def busy_stream(seconds=0.5):
+    """A stream with a wait of the GPU's own on it, and an event behind that."""
+    st, done = torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(st):
+        torch.cuda._sleep(int(seconds * 1.9e9))
+        done.record()
+    return st, done
+
+
+def test_calls_do_not_wait_for_another_threads_sync_errors(R, eng):
+    """While one thread waits for the device in sync_errors, calls of others are enqueued."""
+    q, _ = make_rows(R, eng, "bf16", 20, 128, 1)
+    x, _ = make_rows(R, eng, "bf16", 500, 128, 2)
+    want = R.row_scores(eng, q, x)
+    p = R.score_probs(eng, want, k=3)
+    torch.cuda.synchronize()
+    _, done = busy_stream()
+    waiting = threading.Thread(target=eng.sync_errors)
+    waiting.start()
+    time.sleep(0.1)  # it is inside
+    with torch.cuda.stream(torch.cuda.Stream()):
+        s = R.row_scores(eng, q, x)
+        again = R.score_probs(eng, s, k=3)
+    still_busy = not done.query()
+    waiting.join()
+    assert still_busy
+    assert torch.equal(s, want) and torch.equal(again.top_index, p.top_index)
