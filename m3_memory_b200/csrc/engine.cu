@@ -102,9 +102,18 @@ void encode_tma_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uin
     cuuint64_t gstride[1] = {(cuuint64_t)row_stride_bytes};
     cuuint32_t box[2] = {box_inner, box_rows};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(m, dt, 2, const_cast<void*>(base), gdim, gstride, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return fn(m, dt, 2, const_cast<void*>(base), gdim, gstride, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {  // this host thread's first use of the device
+        int dev = 0;
+        M3G_CK(cudaGetDevice(&dev));
+        M3G_CK(cudaSetDevice(dev));
+        r = encode();
+    }
     if (r != CUDA_SUCCESS)
         fail(M3G_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
 }

@@ -237,3 +237,40 @@ def test_calls_do_not_wait_for_another_threads_sync_errors(R, eng):
     waiting.join()
     assert still_busy
     assert torch.equal(s, want) and torch.equal(again.top_index, p.top_index)
+
+
+def test_first_cuda_call_of_a_host_thread(R, eng):
+    """A thread that has not used CUDA before makes the calls (by their addresses: torch would set
+    the thread up)."""
+    x, xv = make_rows(R, eng, "bf16", 100, 64, 1)
+    out = torch.zeros(100, 100, device="cuda")
+    R.row_scores(eng, x, x)  # its kernel is set up
+    off, length, pairs = T([0]), T([100], torch.int32), T([0, 1])
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    stream, r = st.cuda_stream, cabi.Rows(x.data_ptr(), None, 100, x.stride(0), 0, 64, cabi.BF16)
+    raised = []
+
+    def run(call):
+        def work():
+            try:
+                call()
+            except Exception as e:  # noqa: BLE001
+                raised.append(e)
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert not raised, raised
+
+    run(lambda: eng.row_scores_device(r, r, 1.0, 0.0, out.data_ptr(), cabi.F32, 100, stream))
+    ref, tol = scores_ref(xv, xv, 1.0, 0.0, torch.float32, 64)
+    assert ((out.double() - ref).abs() <= tol).all()
+    R.list_scores(eng, x, x, off, length, pairs, off, out.view(-1))
+    out.zero_()
+    torch.cuda.synchronize()
+    run(lambda: eng.list_scores_device(r, r, 1, off.data_ptr(), length.data_ptr(),
+                                       pairs.data_ptr(), 1, None, off.data_ptr(), 1.0, 0.0,
+                                       out.data_ptr(), cabi.F32, 10000, stream))
+    assert ((out[0].double() - ref[0]).abs() <= tol[0]).all()
+    eng.sync_errors()
