@@ -348,10 +348,12 @@ int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d
  * The calls use no index and no scratch of the engine, so calls on several
  * streams may overlap, and each may be captured into a CUDA graph (make one call
  * of these before the first capture: it allocates the engine's error word).
- * Enqueued on `stream`; stream NULL: the legacy default stream, waited for.  What
- * a kernel finds wrong on the device (a pair, list or row of scores out of range, a
- * wait that gave up) is left out and reported by m3g_sync_errors, or by the call itself
- * when it waits.  Inputs and outputs must not overlap.
+ * Enqueued on `stream`; stream NULL: the legacy default stream, waited for (that
+ * stream alone).  What a kernel finds wrong on the device (a pair, list or row of
+ * scores out of range, a wait that gave up) is left out.  A call that waits reports
+ * what its own kernels found; what those of enqueued calls found, replayed ones too, is
+ * the engine's: the next m3g_sync_errors of any thread reports it, once.  Inputs and
+ * outputs must not overlap.
  *
  * Rows of vectors, one row every `ld` elements:
  *   M3G_BF16  data holds uint16 bf16 bit patterns; scales is not used;

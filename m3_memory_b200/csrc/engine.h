@@ -350,12 +350,15 @@ class Engine {
     std::string first_error_;
     int first_error_code_ = 0;
 
-    // error words of the row-score calls (kScoreErrWords ints on the device, made by
+    // error words of the row-score calls (2 kScoreErrWords ints on the device, made by
     // the first call, under score_mu_; later ones take no lock); row_score_errors()
-    // reads and clears them, one caller at a time
+    // reads and clears those of enqueued calls, one caller at a time.  launch_scores
+    // makes a call's launch: enqueued, or (no stream) waited for, with words of its own
     int* score_err();
     void row_score_errors();
-    std::mutex score_mu_, score_read_mu_;
+    template <class F>
+    void launch_scores(cudaStream_t ext_stream, F launch);
+    std::mutex score_mu_, score_read_mu_, score_wait_mu_;
     DBuf<int> score_words_;
     std::atomic<int*> score_err_{nullptr};  // score_words_, once they are cleared
 

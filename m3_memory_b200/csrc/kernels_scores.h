@@ -11,7 +11,8 @@ namespace m3g {
 
 constexpr int kScaleDims = 128;  // dims that share one scale byte
 
-// Error words of the row-score calls (one pair per engine).
+// Error words of the row-score calls: a pair for an engine's enqueued calls, and one for
+// those that wait (one at a time).
 enum ScoreError : int { kScoreTimeout = 0, kScoreBadItem = 1, kScoreErrWords = 2 };
 
 // The group form's lists and pairs (all null / 0 in the dense form).

@@ -64,6 +64,12 @@ float lowest_score(float c) {
     return t;
 }
 
+void fail_on(const int* w) {
+    if (w[kScoreTimeout]) fail(M3G_ETIMEOUT, "row scores: a device-side wait gave up");
+    if (w[kScoreBadItem])
+        fail(M3G_ERANGE, "row scores: a list, pair or row of scores out of range was left out");
+}
+
 }  // namespace
 
 int* Engine::score_err() {
@@ -71,8 +77,8 @@ int* Engine::score_err() {
     std::lock_guard lk(score_mu_);
     if (!score_err_.load()) {
         DBuf<int> w;
-        w.alloc(kScoreErrWords);
-        M3G_CK(cudaMemset(w.p, 0, kScoreErrWords * sizeof(int)));
+        w.alloc(2 * kScoreErrWords);
+        M3G_CK(cudaMemset(w.p, 0, 2 * kScoreErrWords * sizeof(int)));
         M3G_CK(cudaStreamSynchronize(cudaStreamLegacy));
         score_words_.swap(w);
         score_err_ = score_words_.p;
@@ -88,9 +94,24 @@ void Engine::row_score_errors() {
     int w[kScoreErrWords];
     M3G_CK(cudaMemcpy(w, words, sizeof(w), cudaMemcpyDeviceToHost));
     if (w[kScoreTimeout] || w[kScoreBadItem]) M3G_CK(cudaMemset(words, 0, sizeof(w)));
-    if (w[kScoreTimeout]) fail(M3G_ETIMEOUT, "row scores: a device-side wait gave up");
-    if (w[kScoreBadItem])
-        fail(M3G_ERANGE, "row scores: a list, pair or row of scores out of range was left out");
+    fail_on(w);
+}
+
+template <class F>
+void Engine::launch_scores(cudaStream_t ext, F launch) {
+    int* words = score_err();
+    if (ext) {
+        M3G_CK(launch(words));
+        return;
+    }
+    std::lock_guard lk(score_wait_mu_);
+    words += kScoreErrWords;
+    M3G_CK(launch(words));
+    M3G_CK(cudaStreamSynchronize(ext));
+    int w[kScoreErrWords];
+    M3G_CK(cudaMemcpy(w, words, sizeof(w), cudaMemcpyDeviceToHost));
+    if (w[kScoreTimeout] || w[kScoreBadItem]) M3G_CK(cudaMemset(words, 0, sizeof(w)));
+    fail_on(w);
 }
 
 void Engine::pack_rows(const void* dX, int dtype, int64_t n, int dim, int64_t ldx,
@@ -119,9 +140,9 @@ void Engine::row_scores(const m3g_rows* q, const m3g_rows* x, float alpha, float
     if (q->n == 0 || x->n == 0) return;
     check_out("row_scores", d_out, out_dtype);
     DeviceGuard g(device_);
-    M3G_CK(launch_row_scores(*q, *x, alpha, beta, d_out, out_dtype, ld_out, score_err(), num_sms_,
-                             ext));
-    if (!ext) row_score_errors();
+    launch_scores(ext, [&](int* err) {
+        return launch_row_scores(*q, *x, alpha, beta, d_out, out_dtype, ld_out, err, num_sms_, ext);
+    });
 }
 
 void Engine::list_scores(const m3g_rows* q, const m3g_rows* x, const ScoreGroups& groups,
@@ -139,9 +160,9 @@ void Engine::list_scores(const m3g_rows* q, const m3g_rows* x, const ScoreGroups
         fail(M3G_EINVAL, "list_scores: misaligned buffers");
     check_out("list_scores", d_out, out_dtype);
     DeviceGuard g(device_);
-    M3G_CK(launch_list_scores(*q, *x, s, alpha, beta, d_out, out_dtype, score_err(), num_sms_,
-                              ext));
-    if (!ext) row_score_errors();
+    launch_scores(ext, [&](int* err) {
+        return launch_list_scores(*q, *x, s, alpha, beta, d_out, out_dtype, err, num_sms_, ext);
+    });
 }
 
 int64_t Engine::score_probs_work(int64_t nq, int64_t n, bool ragged, int dtype, int k) {
@@ -179,9 +200,10 @@ void Engine::score_probs(ProbsArgs a, int64_t work_bytes, cudaStream_t ext) {
                              " bytes on an 8-byte boundary");
     DeviceGuard g(device_);
     a.lowest = lowest_score(std::fabs(a.scale));
-    a.err = score_err();
-    M3G_CK(launch_score_probs(a, num_sms_, ext));
-    if (!ext) row_score_errors();
+    launch_scores(ext, [&](int* err) {
+        a.err = err;
+        return launch_score_probs(a, num_sms_, ext);
+    });
 }
 
 }  // namespace m3g

@@ -273,4 +273,77 @@ def test_first_cuda_call_of_a_host_thread(R, eng):
                                        pairs.data_ptr(), 1, None, off.data_ptr(), 1.0, 0.0,
                                        out.data_ptr(), cabi.F32, 10000, stream))
     assert ((out[0].double() - ref[0]).abs() <= tol[0]).all()
+
+
+def plain_call(eng, x, out):
+    """row_scores of bf16 rows without a stream: the call waits."""
+    r = cabi.Rows(x.data_ptr(), None, x.shape[0], x.stride(0), 0, x.shape[1], cabi.BF16)
+    eng.row_scores_device(r, r, 1.0, 0.0, out.data_ptr(), cabi.F32, out.stride(0))
+
+
+def bad_lists(R, eng, x, out):
+    """An enqueued call with a list past the rows."""
+    R.list_scores(eng, x, x, T([0]), T([x.shape[0] + 1], torch.int32), T([0, 1]), T([0]), out)
+
+
+def test_waiting_call_waits_for_its_stream_alone(R, eng):
+    x, xv = make_rows(R, eng, "bf16", 100, 64, 1)
+    out = torch.zeros(100, 100, device="cuda")
+    plain_call(eng, x, out)
+    still_busy = 0
+    for _ in range(6):  # (streams that share a hardware queue do wait for one another)
+        _, done = busy_stream(0.1)
+        plain_call(eng, x, out)
+        still_busy += not done.query()
+        torch.cuda.synchronize()
+    assert still_busy > 0
+    ref, tol = scores_ref(xv, xv, 1.0, 0.0, torch.float32, 64)
+    assert ((out.double() - ref).abs() <= tol).all()
+
+
+def test_waiting_call_reports_its_own_errors_alone(R, eng):
+    x, _ = make_rows(R, eng, "bf16", 100, 64, 1)
+    out = torch.zeros(100, 100, device="cuda")
+    bad_lists(R, eng, x, out.view(-1))
+    torch.cuda.synchronize()
+    plain_call(eng, x, out)  # nothing wrong with this one
+    with pytest.raises(IndexError):
+        eng.sync_errors()
+    # and what a waiting call raised is not reported again
+    r = cabi.Rows(x.data_ptr(), None, 100, x.stride(0), 0, 64, cabi.BF16)
+    off, length, pairs = T([0]), T([101], torch.int32), T([0, 1])
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with pytest.raises(IndexError):
+            eng.list_scores_device(r, r, 1, off.data_ptr(), length.data_ptr(), pairs.data_ptr(), 1,
+                                   None, off.data_ptr(), 1.0, 0.0, out.data_ptr(), cabi.F32, 10000)
+        plain_call(eng, x, out)
+    eng.sync_errors()
+
+
+def test_waiting_calls_of_several_threads(R, eng):
+    """Each raises for itself: the bad ones always, the good ones never."""
+    x, _ = make_rows(R, eng, "bf16", 100, 64, 1)
+    outs = [torch.zeros(100, 100, device="cuda") for _ in range(4)]
+    r = cabi.Rows(x.data_ptr(), None, 100, x.stride(0), 0, 64, cabi.BF16)
+    off, length, pairs = T([0]), T([101], torch.int32), T([0, 1])
+    torch.cuda.synchronize()
+    raised = [0] * 4
+
+    def work(i):
+        for _ in range(50):
+            try:
+                if i % 2:
+                    eng.list_scores_device(r, r, 1, off.data_ptr(), length.data_ptr(),
+                                           pairs.data_ptr(), 1, None, off.data_ptr(), 1.0, 0.0,
+                                           outs[i].data_ptr(), cabi.F32, 10000)
+                else:
+                    plain_call(eng, x, outs[i])
+            except IndexError:
+                raised[i] += 1
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert raised == [0, 50, 0, 50]
     eng.sync_errors()
