@@ -350,9 +350,9 @@ class Engine {
     std::string first_error_;
     int first_error_code_ = 0;
 
-    // error words of the row-score calls (2 kScoreErrWords ints on the device, made by
+    // error words of the row-score calls (3 kScoreErrWords ints on the device, made by
     // the first call, under score_mu_; later ones take no lock); row_score_errors()
-    // reads and clears those of enqueued calls, one caller at a time.  launch_scores
+    // takes those of enqueued calls, one caller at a time.  launch_scores
     // makes a call's launch: enqueued, or (no stream) waited for, with words of its own
     int* score_err();
     void row_score_errors();

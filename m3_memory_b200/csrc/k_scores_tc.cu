@@ -929,7 +929,17 @@ Params params_of(const m3g_rows& q, const m3g_rows& x, float alpha, float beta, 
     return p;
 }
 
+__global__ void take_score_errors_kernel(int* words, int* taken) {
+    if (threadIdx.x < kScoreErrWords)
+        taken[threadIdx.x] = atomicExch(words + threadIdx.x, 0);
+}
+
 }  // namespace
+
+cudaError_t launch_take_score_errors(int* words, int* taken, cudaStream_t st) {
+    take_score_errors_kernel<<<1, 32, 0, st>>>(words, taken);
+    return cudaGetLastError();
+}
 
 cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
                               void* out, int out_dtype, int64_t ld_out, int* err, int sms,

@@ -11,9 +11,12 @@ namespace m3g {
 
 constexpr int kScaleDims = 128;  // dims that share one scale byte
 
-// Error words of the row-score calls: a pair for an engine's enqueued calls, and one for
-// those that wait (one at a time).
+// Error words of the row-score calls: a pair for an engine's enqueued calls, one for
+// those that wait (one at a time), and one to which the first are taken.
 enum ScoreError : int { kScoreTimeout = 0, kScoreBadItem = 1, kScoreErrWords = 2 };
+
+// Moves a pair of words, leaving zeros: kernels that set them meanwhile lose none.
+cudaError_t launch_take_score_errors(int* words, int* taken, cudaStream_t st);
 
 // The group form's lists and pairs (all null / 0 in the dense form).
 struct ScoreGroups {

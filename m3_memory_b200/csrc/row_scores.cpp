@@ -77,8 +77,8 @@ int* Engine::score_err() {
     std::lock_guard lk(score_mu_);
     if (!score_err_.load()) {
         DBuf<int> w;
-        w.alloc(2 * kScoreErrWords);
-        M3G_CK(cudaMemset(w.p, 0, 2 * kScoreErrWords * sizeof(int)));
+        w.alloc(3 * kScoreErrWords);
+        M3G_CK(cudaMemset(w.p, 0, 3 * kScoreErrWords * sizeof(int)));
         M3G_CK(cudaStreamSynchronize(cudaStreamLegacy));
         score_words_.swap(w);
         score_err_ = score_words_.p;
@@ -91,9 +91,10 @@ void Engine::row_score_errors() {
     if (!words) return;
     std::lock_guard lk(score_read_mu_);
     M3G_CK(cudaDeviceSynchronize());
+    int* taken = words + 2 * kScoreErrWords;
+    M3G_CK(launch_take_score_errors(words, taken, cudaStreamLegacy));
     int w[kScoreErrWords];
-    M3G_CK(cudaMemcpy(w, words, sizeof(w), cudaMemcpyDeviceToHost));
-    if (w[kScoreTimeout] || w[kScoreBadItem]) M3G_CK(cudaMemset(words, 0, sizeof(w)));
+    M3G_CK(cudaMemcpy(w, taken, sizeof(w), cudaMemcpyDeviceToHost));
     fail_on(w);
 }
 

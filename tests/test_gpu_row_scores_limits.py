@@ -347,3 +347,36 @@ def test_waiting_calls_of_several_threads(R, eng):
     [t.join() for t in ts]
     assert raised == [0, 50, 0, 50]
     eng.sync_errors()
+
+
+def test_no_error_of_concurrent_calls_is_lost(R, eng):
+    """Bad calls, one after another, while another thread takes errors all the time: after each has
+    ended, an error is reported once more (two calls between two reports share one)."""
+    x, _ = make_rows(R, eng, "bf16", 100, 64, 1)
+    out = torch.zeros(10000, device="cuda")
+    bad_lists(R, eng, x, out)
+    with pytest.raises(IndexError):
+        eng.sync_errors()
+    reports, stop = [0], [False]
+
+    def take():
+        while not stop[0]:
+            try:
+                eng.sync_errors()
+            except IndexError:
+                reports[0] += 1
+
+    t = threading.Thread(target=take)
+    t.start()
+    try:
+        for i in range(300):
+            before = reports[0]
+            bad_lists(R, eng, x, out)
+            deadline = time.time() + 10
+            while reports[0] == before and time.time() < deadline:
+                time.sleep(1e-5)
+            assert reports[0] > before, i
+    finally:
+        stop[0] = True
+        t.join()
+    eng.sync_errors()
