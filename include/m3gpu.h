@@ -346,8 +346,8 @@ int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d
  * No counterpart in the reference, whose searches return the best k scores only
  * and whose rows are fp32.  All arrays are device memory of the engine's device.
  * The calls use no index and no scratch of the engine, so calls on several
- * streams may overlap, and each may be captured into a CUDA graph (make one call
- * of these before the first capture: it allocates the engine's error word).
+ * streams may overlap, and each may be captured into a CUDA graph (an engine's first
+ * one too; the graph is not replayed after the engine is destroyed).
  * Enqueued on `stream`; stream NULL: the legacy default stream, waited for (that
  * stream alone).  What a kernel finds wrong on the device (a pair, list or row of
  * scores out of range, a wait that gave up) is left out.  A call that waits reports

@@ -64,6 +64,18 @@ float lowest_score(float c) {
     return t;
 }
 
+// This thread's allocations and waits are allowed while a stream captures.
+struct CaptureRelaxed {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    CaptureRelaxed() { M3G_CK(cudaThreadExchangeStreamCaptureMode(&mode)); }
+    ~CaptureRelaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+struct OwnStream {
+    cudaStream_t st = nullptr;
+    OwnStream() { M3G_CK(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking)); }
+    ~OwnStream() { cudaStreamDestroy(st); }
+};
+
 void fail_on(const int* w) {
     if (w[kScoreTimeout]) fail(M3G_ETIMEOUT, "row scores: a device-side wait gave up");
     if (w[kScoreBadItem])
@@ -76,10 +88,13 @@ int* Engine::score_err() {
     if (int* words = score_err_.load()) return words;
     std::lock_guard lk(score_mu_);
     if (!score_err_.load()) {
+        // (on a stream of its own: the call may be captured, by another stream's capture)
+        CaptureRelaxed relaxed;
         DBuf<int> w;
         w.alloc(3 * kScoreErrWords);
-        M3G_CK(cudaMemset(w.p, 0, 3 * kScoreErrWords * sizeof(int)));
-        M3G_CK(cudaStreamSynchronize(cudaStreamLegacy));
+        OwnStream st;
+        M3G_CK(cudaMemsetAsync(w.p, 0, 3 * kScoreErrWords * sizeof(int), st.st));
+        M3G_CK(cudaStreamSynchronize(st.st));
         score_words_.swap(w);
         score_err_ = score_words_.p;
     }

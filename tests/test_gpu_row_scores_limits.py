@@ -380,3 +380,48 @@ def test_no_error_of_concurrent_calls_is_lost(R, eng):
         stop[0] = True
         t.join()
     eng.sync_errors()
+
+
+# ---------------- first calls within a capture ----------------
+
+
+@pytest.mark.parametrize("warm_up", ["none", "pack", "empty"])
+@pytest.mark.parametrize("what", ["scores", "lists", "probs"])
+def test_first_call_of_an_engine_is_captured(R, what, warm_up):
+    """A new engine's first call, or its first after packing or an empty call, is made in a
+    capture: the graph holds it and reports through the engine."""
+    e = cabi.Engine()
+    n, dim, nq = 300, 128, 9
+    x, xv = make_rows(R, cabi.Engine(), "e4m3", n, dim, 1)
+    q, qv = make_rows(R, cabi.Engine(), "e4m3", nq, dim, 2)
+    if warm_up == "pack":
+        R.pack_rows(e, torch.randn(5, dim, device="cuda"))
+    elif warm_up == "empty":
+        R.row_scores(e, R.PackedRows(q.codes[:0], q.scales[:0], dim), x)
+    out = torch.zeros(nq, n, device="cuda")
+    off, length, pairs = T([0]), T([n], torch.int32), T([0, nq])
+    at = torch.arange(nq, device="cuda") * n
+    s = torch.randn(3, 60001, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        if what == "scores":
+            R.row_scores(e, q, x, out=out)
+        elif what == "lists":
+            R.list_scores(e, q, x, off, length, pairs, at, out.view(-1))
+        else:
+            got = R.score_probs(e, s, k=5)
+    g.replay()
+    torch.cuda.synchronize()
+    if what == "probs":
+        assert torch.equal(got.top_index, R.score_probs(e, s, k=5).top_index)
+    else:
+        ref, tol = scores_ref(qv, xv, 1.0, 0.0, torch.float32, dim)
+        assert ((out.double() - ref).abs() <= tol).all()
+    e.sync_errors()
+    if what == "lists":
+        length.fill_(n + 1)
+        g.replay()
+        with pytest.raises(IndexError):
+            e.sync_errors()
+    del g
