@@ -276,9 +276,10 @@ __device__ __forceinline__ void store_columns(O* mine, int64_t ld, uint32_t acc,
 }
 
 // A group's tiles: its rows in 128s (nx) times its pairs in nqt parts of `per`, the
-// pairs fastest.  CTAs take runs of equal weight: a tile of 32 b rows weighs 1 + 2 b
-// with few queries, where loading it is most of its time, and the same always with
-// many, where the MMAs are.
+// pairs fastest.  CTAs take runs of equal weight: with few queries, where loading it is
+// most of its time, a tile of 128 rows weighs 9 and a list's last one, of r rows,
+// 1 + (r + 31) / 16 (whole numbers: 3 to 10; by 32-row boxes, 1 + 2 ceil(r / 32), 4096 x
+// 16 of 4096 lists took 266 us for 263); the same always with many, where the MMAs are.
 template <int NT>
 struct Tiles {
     int64_t nx;
@@ -295,7 +296,7 @@ struct Tiles {
         per = (int32_t)max((n + 15u) & ~15u, 16u);
         nqt = n == (uint32_t)m ? 1 : (int32_t)(((uint32_t)m + per - 1) / (uint32_t)per);
         w = NT > 64 ? 1 : 9;
-        wlast = NT > 64 ? 1 : 1 + 2 * ((int32_t)(len - (nx - 1) * kM) + 31) / 32;
+        wlast = NT > 64 ? 1 : 1 + ((int32_t)(len - (nx - 1) * kM) + 31) / 16;
     }
     __device__ __forceinline__ int64_t count() const { return nx * nqt; }
     __device__ __forceinline__ int64_t weight() const {
