@@ -8,7 +8,9 @@ the reference, whose searches return k scores (AgentMemory/M3/src/m3_index.cpp:4
 
 Every call is enqueued on the current torch stream and returns at once; ``Engine.sync_errors()``
 reports what a kernel found wrong (see include/m3gpu.h, which states the formulas).  Rows are bf16
-tensors ``[n, dim]`` or ``PackedRows``; a tensor's rows must start on 16-byte boundaries.
+tensors ``[n, dim]`` or ``PackedRows``; a tensor's rows must start on 16-byte boundaries.  There are
+no backward forms: a tensor that requires a gradient is refused (detach it, or call under
+``torch.no_grad()``).
 """
 from __future__ import annotations
 
@@ -78,8 +80,16 @@ def _bad(what, msg):
     raise ValueError(f"{what} {msg}")
 
 
+def _no_grad(t, what):
+    if t.requires_grad and torch.is_grad_enabled():
+        _bad(what, "requires a gradient, which these calls do not give")
+
+
 def _device_of(engine, t, what):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, torch.Tensor):
+        _bad(what, "must be a CUDA tensor")
+    _no_grad(t, what)
+    if not t.is_cuda:
         _bad(what, "must be a CUDA tensor")
     dev = t.get_device()
     if dev != engine.device():
@@ -129,6 +139,7 @@ def _rows(r, dev, what):
         return cabi.Rows(codes.data_ptr(), scales.data_ptr(), n, ld, lds, dim, cabi.E4M3)
     if not isinstance(r, torch.Tensor) or r.dtype != _BF16:
         _bad(what, "must be PackedRows or a bf16 tensor")
+    _no_grad(r, what)
     n, dim, ld = _matrix(r, dev, what)
     if n <= 1:
         ld = (dim + 7) // 8 * 8
@@ -176,6 +187,7 @@ def row_scores(engine, q, x, alpha=1.0, beta=0.0, out_dtype=torch.float32, out=N
         out = _matrix_of(a.n, b.n, out_dtype, t.device)
         ld = b.n
     else:
+        _no_grad(out, "out")
         n, d, ld = _matrix(out, dev, "out")
         if n != a.n or d != b.n:
             _bad("out", f"must be [{a.n}, {b.n}]")
@@ -196,6 +208,7 @@ def list_scores(engine, q, x, list_off, list_len, pair_off, out_off, out, pair_r
     dev = _device(engine, x, "x")
     a, b = _rows(q, dev, "q"), _rows(x, dev, "x")
     ngroup, npair, n = list_off.numel(), out_off.numel(), out.numel()
+    _no_grad(out, "out")
     engine.list_scores_device(
         a, b, ngroup, _vector(list_off, _I64, ngroup, dev, "list_off"),
         _vector(list_len, _I32, ngroup, dev, "list_len"),
