@@ -144,9 +144,9 @@ __global__ void __launch_bounds__(256)
 
 template <class T>
 void launch_typed(const T* x, int64_t n, int dim, int64_t ldx, uint8_t* codes, int64_t ld,
-                  uint8_t* scales, int64_t lds, cudaStream_t st) {
+                  uint8_t* scales, int64_t lds, int sms, cudaStream_t st) {
     const int nblk = (dim + kScaleDims - 1) / kScaleDims;
-    const unsigned grid = (unsigned)std::min<int64_t>((n * nblk + 31) / 32, 148 * 4);
+    const unsigned grid = (unsigned)std::min<int64_t>((n * nblk + 31) / 32, sms * 4);
     if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && ldx * sizeof(T) % 16 == 0)
         pack_rows_kernel<T, true><<<grid, 256, 0, st>>>(x, n, dim, ldx, nblk, codes, ld, scales,
                                                         lds);
@@ -158,13 +158,14 @@ void launch_typed(const T* x, int64_t n, int dim, int64_t ldx, uint8_t* codes, i
 }  // namespace
 
 cudaError_t launch_pack_rows(const void* x, int dtype, int64_t n, int dim, int64_t ldx,
-                             uint8_t* codes, int64_t ld, uint8_t* scales, int64_t lds,
+                             uint8_t* codes, int64_t ld, uint8_t* scales, int64_t lds, int sms,
                              cudaStream_t st) {
     if (dtype == M3G_F32)
-        launch_typed(static_cast<const float*>(x), n, dim, ldx, codes, ld, scales, lds, st);
+        launch_typed(static_cast<const float*>(x), n, dim, ldx, codes, ld, scales, lds, sms,
+                     st);
     else
         launch_typed(static_cast<const __nv_bfloat16*>(x), n, dim, ldx, codes, ld, scales, lds,
-                     st);
+                     sms, st);
     return cudaGetLastError();
 }
 

@@ -29,7 +29,7 @@ struct ScoreGroups {
 };
 
 cudaError_t launch_pack_rows(const void* x, int dtype, int64_t n, int dim, int64_t ldx,
-                             uint8_t* codes, int64_t ld, uint8_t* scales, int64_t lds,
+                             uint8_t* codes, int64_t ld, uint8_t* scales, int64_t lds, int sms,
                              cudaStream_t st);
 cudaError_t launch_row_scores(const m3g_rows& q, const m3g_rows& x, float alpha, float beta,
                               void* out, int out_dtype, int64_t ld_out, int* err, int sms,

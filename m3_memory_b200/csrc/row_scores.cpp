@@ -144,7 +144,7 @@ void Engine::pack_rows(const void* dX, int dtype, int64_t n, int dim, int64_t ld
     DeviceGuard g(device_);
     M3G_CK(launch_pack_rows(dX, dtype, n, dim, ldx,
                             static_cast<uint8_t*>(const_cast<void*>(out->data)), out->ld,
-                            const_cast<uint8_t*>(out->scales), out->ld_scales, ext));
+                            const_cast<uint8_t*>(out->scales), out->ld_scales, num_sms_, ext));
     if (!ext) M3G_CK(cudaStreamSynchronize(ext));
 }
 
