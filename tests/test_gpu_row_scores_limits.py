@@ -425,3 +425,137 @@ def test_first_call_of_an_engine_is_captured(R, what, warm_up):
         with pytest.raises(IndexError):
             e.sync_errors()
     del g
+
+
+# ---------------- sizes ----------------
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 7, 8, 9, 15, 17, 31, 33, 63, 65, 20001])
+@pytest.mark.parametrize("kind", ["e4m3", "bf16"])
+def test_rows_of_few_and_of_many_dims(R, eng, kind, dim):
+    q, qv = make_rows(R, eng, kind, 70, dim, 1, gap=1)
+    x, xv = make_rows(R, eng, kind, 200, dim, 2, gap=1)
+    ref, tol = scores_ref(qv, xv, 1.0, 0.0, torch.float32, dim)
+    assert ((R.row_scores(eng, q, x).double() - ref).abs() <= tol).all()
+    for gather in (True, False):
+        out = torch.full((70, 200), 7.0, device="cuda")
+        R.list_scores(eng, q, x, T([0]), T([200], torch.int32), T([0, 70]),
+                      torch.arange(70, device="cuda") * 200, out.view(-1),
+                      pair_row=torch.arange(70, device="cuda").int() if gather else None)
+        assert ((out.double() - ref).abs() <= tol).all()
+    eng.sync_errors()
+
+
+@pytest.mark.parametrize("nlist", [300001, 1 << 22])
+def test_many_lists(R, eng, nlist):
+    """Most lists empty or not probed; the last one and every 1009th are."""
+    dim, n, nq = 64, 5000, 12
+    q, qv = make_rows(R, eng, "e4m3", nq, dim, 1)
+    x, xv = make_rows(R, eng, "e4m3", n, dim, 2)
+    g = torch.arange(nlist, device="cuda")
+    probed = (g % 1009 == 0) | (g == nlist - 1)
+    length = (g * 7 % 5).int()
+    off = g * 31 % (n - 5)
+    pair_off = torch.cat([T([0]), probed.long().cumsum(0)])
+    group = probed.nonzero()[:, 0]
+    npair = len(group)
+    row = torch.arange(npair, device="cuda") % nq
+    size = length[group].long()
+    start = size.cumsum(0) - size
+    out = torch.full((int(size.sum()),), 7.0, device="cuda")
+    R.list_scores(eng, q, x, off, length, pair_off, start, out, pair_row=row.int())
+    eng.sync_errors()
+    pair = torch.repeat_interleave(torch.arange(npair, device="cuda"), size)
+    j = torch.arange(len(pair), device="cuda") - start[pair]
+    a, b = qv[row[pair]], xv[off[group[pair]] + j]
+    tol = (dim + 2) * 2 * U32 * 1.01 * (a.abs() * b.abs()).sum(1)  # (see scores_ref)
+    assert ((out.double() - (a * b).sum(1)).abs() <= tol + 2 * U32 * (a * b).sum(1).abs()).all()
+
+
+FAR = (1 << 32) + 24  # elements: past what 32 bits hold, a multiple of 8
+
+
+def test_outputs_and_scores_past_32_bits(R, eng):
+    """Rows of scores more than 2^32 elements apart, written and read there."""
+    nq, n, dim = 2, 700, 96
+    q, qv = make_rows(R, eng, "bf16", nq, dim, 1)
+    x, xv = make_rows(R, eng, "bf16", n, dim, 2)
+    store = torch.empty(FAR + n, dtype=torch.bfloat16, device="cuda")
+    out = store.as_strided((nq, n), (FAR, 1))
+    R.row_scores(eng, q, x, out=out)
+    ref, tol = scores_ref(qv, xv, 1.0, 0.0, torch.bfloat16, dim)
+    assert ((out.double() - ref).abs() <= tol).all()
+    got = R.score_probs(eng, out, scale=0.01, k=5)
+    near = R.score_probs(eng, out.contiguous(), scale=0.01, k=5)
+    assert all(torch.equal(a, b) for a, b in zip((got.logsumexp, got.entropy, got.top_index),
+                                                 (near.logsumexp, near.entropy, near.top_index)))
+    # as lists: a pair's scores that start past 2^32, and a ragged row there
+    store.view(-1)[FAR:] = 7.0
+    R.list_scores(eng, q, x, T([0]), T([n], torch.int32), T([0, 1]), T([FAR]), store,
+                  pair_row=T([1], torch.int32))
+    assert ((store[FAR:].double() - ref[1]).abs() <= tol[1]).all()
+    far = R.score_probs(eng, store, scale=0.01, k=5, row_off=T([FAR, FAR + n]))
+    assert torch.equal(far.top_index[0], near.top_index[1])
+    eng.sync_errors()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "bf16"])
+def test_rows_past_32_bits(R, eng, kind):
+    """Rows (and their scales) more than 2^32 bytes from the first, packed, scored and gathered."""
+    dim, n, nq = 128, 3, 20
+    ld = 1 << 31
+    v = torch.randn(n, dim, device="cuda")
+    if kind == "e4m3":
+        src = torch.empty((n - 1) * ld + dim, dtype=torch.bfloat16, device="cuda").as_strided(
+            (n, dim), (ld, 1))
+        src.copy_(v)
+        codes = torch.empty((n - 1) * ld * 2 + dim, dtype=torch.uint8,
+                            device="cuda").as_strided((n, dim), (2 * ld, 1))
+        scales = torch.empty((n - 1) * ld * 2 + 4, dtype=torch.uint8,
+                             device="cuda").as_strided((n, 4), (2 * ld, 1))
+        x = R.pack_rows(eng, src, out=R.PackedRows(codes, scales, dim))
+        near = R.pack_rows(eng, v.bfloat16())
+        assert torch.equal(codes, near.codes) and torch.equal(scales[:, 0], near.scales[:, 0])
+        q, _ = make_rows(R, eng, kind, nq, dim, 3)
+    else:
+        near = v.bfloat16()
+        x = torch.empty((n - 1) * ld + dim, dtype=torch.bfloat16, device="cuda").as_strided(
+            (n, dim), (ld, 1))
+        x.copy_(near)
+        q, _ = make_rows(R, eng, kind, nq, dim, 3)
+    assert torch.equal(R.row_scores(eng, q, x), R.row_scores(eng, q, near))
+    assert torch.equal(R.row_scores(eng, x, q), R.row_scores(eng, near, q))
+    row = torch.arange(2 * n, device="cuda").int() % n
+    outs = []
+    for a in (x, near):
+        out = torch.empty(2 * n * nq, device="cuda")
+        R.list_scores(eng, a, q, T([0]), T([nq], torch.int32), T([0, 2 * n]),
+                      torch.arange(2 * n, device="cuda") * nq, out, pair_row=row)
+        outs.append(out)
+    assert torch.equal(*outs)
+    eng.sync_errors()
+
+
+@pytest.mark.parametrize("dim,pairs", [(96, 300), (513, 40), (640, 300), (1536, 64), (1537, 300),
+                                       (2048, 10), (2048, 300)])
+@pytest.mark.parametrize("gather", [True, False])
+def test_fp32_list_scores_of_bf16_rows_are_not_low(R, eng, dim, pairs, gather):
+    """Sums of like terms in lists, as for every row: what the tensor core cuts off, half a step of
+    fp32 on average every 16 dims of each of the sums (four for up to 64 pairs a list or from 1537
+    dims on, two from 513 on, else one), and fp32 rounding of their sum."""
+    base = torch.randn(1, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(dim))
+    pad = -dim % 8
+
+    def rows(n):
+        v = (base + 0.3 * torch.randn(n, dim, device="cuda")).bfloat16()
+        return torch.nn.functional.pad(v, (0, pad))[:, :dim]
+
+    x, q = rows(700), rows(pairs)
+    out = torch.empty(pairs, 700, device="cuda")
+    R.list_scores(eng, q, x, T([0]), T([700], torch.int32), T([0, pairs]),
+                  torch.arange(pairs, device="cuda") * 700, out.view(-1),
+                  pair_row=torch.arange(pairs, device="cuda").int() if gather else None)
+    want = q.double() @ x.double().t()
+    parts = 4 if pairs <= 64 or dim > 1536 else 2 if dim > 512 else 1
+    low = ((want - out.double()) / want).mean().item()
+    assert abs(low) <= (dim / 16 / parts / 2 + 2) * 2 * U32, low
