@@ -57,8 +57,8 @@ __device__ __forceinline__ float max_of_8_lanes(float m) {
 
 // Eight lanes a block of 128 dims, 16 values a lane in 16-byte loads eight lanes wide
 // (with a lane for each 16 bytes of fp32, four values, the work a block costs beside
-// its values took more time than the bytes: 1396 us where this takes 845); kU blocks
-// in flight a lane.  The bytes bound it: 1M x 1024 fp32 rows at 6.1 TB/s.  VEC: rows on
+// its values took more time than the bytes: 1396 us where this takes 862); kU blocks
+// in flight a lane.  The bytes bound it: 1M x 1024 fp32 rows at 5.9 TB/s.  VEC: rows on
 // 16-byte boundaries; else value by value.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256)

@@ -24,9 +24,9 @@
 // rounds' ceil(k / 8)-th largest.  The buffer is cut to its best k, which sharpens tau,
 // whenever it holds twice as many, and before it could overflow.
 //
-// The scores' bytes bound it without the best k (1024 rows x 100003 fp32: 65 us, 6.3
-// TB/s); the best k add work that each warp does in turn: 85 us for k = 10, 165 for 100;
-// 4096 rows of 3904 bf16 scores 17 us, and 37 and 73.  A row of 1000003 is latency: 9 us
+// The scores' bytes bound it without the best k (1024 rows x 100003 fp32: 67 us, 6.1
+// TB/s); the best k add work that each warp does in turn: 89 us for k = 10, 177 for 100;
+// 4096 rows of 3904 bf16 scores 16 us, and 36 and 73.  A row of 1000003 is latency: 9 us
 // for its 488 parts and 6 to join them, k = 10.  Blocks of 256 threads a row, all of a
 // row's best k through one buffer, took 107 us (k = 0) and 198 (10) for the first shape.
 #include <cuda_bf16.h>

@@ -21,19 +21,20 @@
 // warp 1 issues the MMAs, warp 3 walks the groups and queues tiles, warps 4-11 store,
 // warps 16-19 bring scale words.  Every wait is bounded.
 //
-// What bounds it, and what it measured:
+// What bounds it, and what it measured (launches by themselves; back to back the clock
+// falls, and dense products take up to a tenth longer):
 //   few queries a row: the rows' bytes.  One query against 1M x 1024 8-bit rows 157 us
 //     (6.6 TB/s); 1024 queries x 32 of 4096 lists, 1M x 1024 8-bit rows 186 us (5.5);
 //     4096 x 16 of 4096 lists, 1M x 768 bf16 rows 257 us (5.9; partly filled tiles cost
 //     the MMA warp as much as full ones, and a tile of 8-bit rows has fewer bytes).
-//   many queries: the operands through L2, 46 KB for 128 bytes of K of a 128 x 240 tile
-//     at the 40 bytes a cycle L2 gives an SM, and the scores' own bytes.  1024 queries x
-//     100096 rows x 1024 dims 142 us (1480 TFLOP/s), 4096 x 16384 x 768 bf16 94 us
-//     (1100).  Rows of scores that do not start on 32-byte boundaries cost up to 1.8
-//     times their bytes: every 32-row store ends inside sectors (x 128 dims: 87 us where
-//     n is a multiple of 8, 150 where it is odd).  CTA pairs (cta_group::2, 31 KB of
-//     operands a CTA) took 150 and 88 us, staging the scores through shared memory for
-//     16-byte stores 164: neither was kept.
+//   many queries: the operands through L2, 46 KB for 128 bytes of K of a 128 x 240 tile,
+//     beside the scores' own bytes.  1024 queries x 100096 rows x 1024 dims 142 us (1480
+//     TFLOP/s; 37 bytes of operands a cycle and SM), 4096 x 16384 x 768 bf16 94 us (1100;
+//     49).  CTA pairs (cta_group::2, 31 KB of operands a CTA) took 150 and 88 us, so the
+//     operands are not all of it; staging the scores through shared memory for 16-byte
+//     stores 164: neither was kept.  Rows of scores that do not start on 32-byte
+//     boundaries cost up to twice their time: every 32-row store ends inside sectors (x
+//     128 dims: 83 us for n = 100000, 160 for 100003).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
