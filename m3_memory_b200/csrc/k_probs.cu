@@ -525,19 +525,27 @@ struct Unit {
 };
 
 // A part's n entries from x on, and one a lane besides, summed up again from a reference
-// value in two words; m is their largest score.
+// value in two words; m is their largest score.  In blocks of sixteen a lane, so that a
+// long row's sums lose no more than the first pass's.
 template <class T>
 __device__ __noinline__ Sums sums_of_far(const T* x, int n, float edge, float c, float sgn,
                                          float m) {
     const Ref ref = ref_of(c, m);
     Sums s{m, 0.f, 0.f};
-    auto add = [&](float t) {
+    auto add = [&](float t, float& z, float& w) {
         const float d = fmaxf(from_ref(c, t, ref), -1000.f), e = exp_of(d);
-        s.z += e;
-        s.w = fmaf(e, d, s.w);
+        z += e;
+        w = fmaf(e, d, w);
     };
-    for (int i = threadIdx.x & 31; i < n; i += 32) add(sgn * load_score(x + i));
-    add(sgn * edge);
+    for (int64_t b = threadIdx.x & 31; b < n; b += 32 * 16) {
+        float z = 0.f, w = 0.f;
+#pragma unroll 4
+        for (int u = 0; u < 16; ++u)
+            if (b + 32 * u < n) add(sgn * load_score(x + b + 32 * u), z, w);
+        s.z += z;
+        s.w += w;
+    }
+    add(sgn * edge, s.z, s.w);
     return warp_join<false>(s, c);
 }
 

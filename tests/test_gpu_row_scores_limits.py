@@ -207,6 +207,33 @@ def test_rows_masked_by_a_large_value(R, eng, mask, dtype, scale):
         probs_check(R, eng, s, list(rows), scale, k)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_masked_rows_that_are_not_split(R, eng, dtype):
+    """So many rows that a warp takes each whole: masked runs of long rows, and rows of large
+    logits, sum up as well as other rows (a lane adds n / 512 blocks of at most 16 sums, and the
+    lanes' are joined in 5 steps)."""
+    nq, n, scale = 1800, 60001, float(np.float32(50.3))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    s = torch.randn(nq, n, device="cuda", generator=g) * 0.004
+    s[0, :20000] = -1e9
+    s[1, 40000:] = -1e9
+    s[2, ::2] = -1e30
+    s[3] = 3e8
+    s = s.to(dtype)
+    got = R.score_probs(eng, s, scale=scale, k=2)
+    for i in range(5):
+        l = s[i].double() * scale
+        d = l - l.max()
+        p = d.exp()
+        z, t = p.sum().item(), (p * d).sum().item()
+        adds = (n / 512 + 16 + 5) * U32
+        rel = adds + 2.0 ** -21 + 2.0 ** -22 * abs(t) / z  # (see probs_ref)
+        lse, ent = l.max().item() + np.log(z), np.log(z) - t / z
+        assert abs(got.logsumexp[i].item() - lse) <= rel + 4 * U32 * (abs(lse) + 12.0), i
+        assert abs(got.entropy[i].item() - ent) <= rel * (1 + 2 * abs(t) / z) + 8 * U32 * 12.0, i
+        assert abs(got.top[i, 0].item() + np.log(z)) <= rel + 4 * U32 * 12.0, i
+
+
 # ---------------- several callers ----------------
 
 
