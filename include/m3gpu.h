@@ -352,7 +352,8 @@ int m3g_select_probes_noalloc(const float* d_queries, int64_t nq, const float* d
  * stream alone).  What a kernel finds wrong on the device (a pair, list or row of
  * scores out of range, a wait that gave up) is left out.  A call that waits reports
  * what its own kernels found; what those of enqueued calls found, replayed ones too, is
- * the engine's: the next m3g_sync_errors of any thread reports it, once.  A call without
+ * the engine's: the next m3g_sync_errors of any thread reports it, once (it waits for
+ * the device, which CUDA refuses while any stream captures).  A call without
  * rows, queries, lists, pairs or elements to write does nothing.  Inputs and outputs
  * must not overlap.
  *
